@@ -550,6 +550,153 @@ jk_status jk_host_gemm_i8(const int8_t *a, size_t a_len, size_t m, const int8_t 
                           size_t n1, size_t k, int32_t *c, size_t c_len);
 jk_status jk_host_dot_i8(const int8_t *a, size_t a_len, const int8_t *b, size_t b_len, int32_t *out);
 
+/* ------------------------------------ a batch's paged attention cache in 8 bits */
+/* What stands between a decoder layer's K/V projections and its output projection when a batch of
+ * requests is served: which page each token goes to, the cache, the attention that reads it, and
+ * beam search over it. No reference function corresponds (the reference's attention keeps one
+ * request's cache in f32). All arrays are device memory of the caller; the calls allocate nothing,
+ * synchronize nothing and can be captured in a graph. Lengths, tables and slots are read on the
+ * device: the kernels check every index that they take from there against the sizes given here. */
+
+/* Element types of activations and logits, by their GGML type ids. */
+typedef enum jk_dtype { JK_F32 = 0, JK_F16 = 1, JK_BF16 = 30 } jk_dtype;
+
+/* The pages of a batch. Token t of request r lies in page table[r][t / page], at row t % page. */
+typedef struct jk_paged {
+    size_t n_requests;
+    size_t max_pages; /* columns of the tables */
+    size_t n_pages;   /* pages of the cache; n_pages * page at most 2^31 - 1 */
+    size_t page;      /* tokens a page: 16, 32, 64, 128 or 256 */
+    int32_t *lens;    /* [n_requests] tokens held */
+    int32_t *table;   /* [n_requests][max_pages] page ids; -1 past the pages in use after a reset */
+    int32_t *owned;   /* [n_requests][max_pages] the page allocated for that place by that request, -1 for none.
+                       * The same array as table where requests share no pages (no jk_paged_reorder) */
+    int32_t *free_pages; /* [n_pages] stack of the free page ids */
+    int32_t *n_free;     /* [1] its height */
+} jk_paged;
+
+/* What a step's tokens are and where they go, written by jk_paged_extend. */
+typedef struct jk_paged_step {
+    size_t max_tokens;  /* entries of slots, positions and requests */
+    int32_t *q_start;   /* [n_requests + 1] first token of each request in the step, then the total */
+    int32_t *slots;     /* [max_tokens] page * tokens a page + row; -1 past the step's tokens */
+    int32_t *positions; /* [max_tokens] position in its request (for a rotary embedding); -1 past them */
+    int32_t *requests;  /* [max_tokens] request of each token; -1 past them */
+    int32_t *status;    /* [1] 0, or why nothing was done (jk_paged_status) */
+} jk_paged_step;
+
+typedef enum jk_paged_status {
+    JK_PAGED_OK = 0,
+    JK_PAGED_NO_PAGES = 1,   /* fewer free pages than needed */
+    JK_PAGED_TOO_LONG = 2,   /* a request would pass max_pages pages, or the step max_tokens tokens */
+    JK_PAGED_BAD_LENGTH = 3, /* a negative length or count, a length past max_pages pages, n_free outside 0..n_pages */
+    JK_PAGED_NOT_OWNED = 4   /* jk_paged_reorder: the page that a parent is filling is not its own */
+} jk_paged_status;
+
+/* Empty requests and all pages free: lens = 0, table = owned = -1, and a stack that gives page 0 first. */
+jk_status jk_paged_reset(jk_stream s, const jk_paged *p);
+/* Adds n_new[r] tokens (device, 0 or more) to each request r. Pages that begin in the step are taken
+ * from the top of the stack, request by request. The new lengths and stack height go to lens_out
+ * [n_requests] and n_free_out [1], or back into p where these are NULL; a caller that passes its own
+ * can drop the step (drafted tokens that were refused) by going on from the old ones. The stack itself is only
+ * read. If the step does not fit, status says why and nothing else changes but the step's outputs:
+ * q_start is 0, slots, positions and requests are -1, and lens_out and n_free_out are copies. */
+jk_status jk_paged_extend(jk_stream s, const jk_paged *p, const int32_t *n_new, const jk_paged_step *step,
+                          int32_t *lens_out, int32_t *n_free_out);
+/* Ends the requests r with ended[r] != 0 (device, [n_requests]): their owned pages go back on the stack in
+ * order of request and place, their rows to -1 and their lengths to 0. Requests that share pages
+ * (after jk_paged_reorder) are to be ended together. */
+jk_status jk_paged_release(jk_stream s, const jk_paged *p, const int32_t *ended);
+/* Reordering by a beam search's choice. Requests come in groups of `width` hypotheses (1..32, n_requests a
+ * multiple); row r of a group goes on from row parent[r] of the group (0..width-1; r itself where it
+ * is out of range). Full pages are shared: the row of the table becomes the parent's. The page that is still being
+ * filled becomes a page of the row's own, owned[r][.], taken from the stack if it has none there; its
+ * contents are moved by jk_kv_reorder_q8, once for each layer's cache. Columns past the pages in use
+ * become -1. lens and table go to lens_out and table_out, or back into p where these are NULL (pass both
+ * or neither); owned, the stack's height and status (as jk_paged_step) are in place. p->owned and
+ * p->table must be different arrays. */
+jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent, size_t width, int32_t *status,
+                           int32_t *lens_out, int32_t *table_out);
+
+/* One layer's cache. Codes of page p, kv head h, row t and channel d at ((p * n_kv + h) * page + t) * head_dim + d;
+ * a value is code * scale[p * n_kv + h]. */
+typedef struct jk_kv_q8 {
+    size_t n_pages, page; /* as in jk_paged */
+    size_t n_kv;          /* kv heads */
+    size_t head_dim;      /* a multiple of 16, 16..256 */
+    int8_t *k, *v;        /* 16-byte aligned */
+    float *k_scale, *v_scale;
+} jk_kv_q8;
+
+/* Quantizes n_tokens keys and values into their slots. x[t][h][d] lies at t * stride_token + h * stride_head + d
+ * (elements; strides of 0: packed). A page's scale d is (largest finite |x| of its tokens) / 127, and its
+ * codes are round(x / d) with x * (1 / d) in f32, ties to even. A page that was begun earlier keeps its scale while it
+ * suffices; when a larger value comes, its older codes become round(code * (d_old / d)). Its row 0
+ * begins a page anew. Non-finite values are stored as 0, and so is a page whose largest value is below 2^-119.
+ * The tokens of one page have to be neighbours in the step, in the order of their rows (as jk_paged_extend
+ * numbers them); slots out of range, -1 among them, are skipped. */
+jk_status jk_kv_append_q8(jk_stream s, const jk_kv_q8 *c, const void *k, const void *v, int dtype, size_t n_tokens,
+                          size_t stride_token, size_t stride_head, const int32_t *slots);
+/* The values that n slots hold, k_out and v_out [n][n_kv][head_dim]; 0 for slots out of range. Either may be NULL. */
+jk_status jk_kv_read_q8(jk_stream s, const jk_kv_q8 *c, const int32_t *slots, size_t n, int dtype, void *k_out,
+                        void *v_out);
+/* The cache's part of jk_paged_reorder, after it and for each layer: the parent's rows of the page that is
+ * still being filled, and its scales, into the row's own page. p's lens are those after the reorder; status
+ * is what jk_paged_reorder wrote (where it is not 0 nothing is moved). */
+jk_status jk_kv_reorder_q8(jk_stream s, const jk_kv_q8 *c, const jk_paged *p, const int32_t *parent, size_t width,
+                           const int32_t *status);
+
+/* Causal attention of a step's queries over the cache. Token i of request r is query
+ * q_start[r] + i and stands at position pos = lens[r] - (q_start[r+1] - q_start[r]) + i: it sees the tokens j with
+ * j <= pos and, with a window, j > pos - window. o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - max). Query
+ * head h reads kv head h / (n_heads / n_kv). A query that sees nothing gives 0. */
+typedef struct jk_attn_q8_args {
+    const void *q; /* [t][n_heads][head_dim], strides in elements (0: packed), as out */
+    void *out;
+    int32_t dtype; /* jk_dtype of q and out */
+    size_t n_tokens; /* rows of q and out; those that q_start gives to no request are left as they are */
+    size_t n_heads;  /* a multiple of n_kv */
+    size_t q_stride_token, q_stride_head, out_stride_token, out_stride_head;
+    size_t n_requests, max_pages;
+    const int32_t *q_start; /* [n_requests + 1] */
+    const int32_t *lens;    /* [n_requests], the step's tokens included; not past max_pages * page */
+    const int32_t *table;   /* [n_requests][max_pages] */
+    size_t max_new; /* bound of the new tokens of one request: later ones are left as they are */
+    size_t max_len; /* expected bound of lens: work is split by it, results do not depend on it */
+    float scale;
+    size_t window; /* 0: none */
+} jk_attn_q8_args;
+/* Queries of f32 are multiplied as two f16 parts (22 bits of each row's largest value) and so are the
+ * probabilities; f16 and bf16 queries are exact (to 2^-24 of their row's largest value), with
+ * probabilities in f16. Scores, maxima, sums and outputs are f32 until the one rounding to dtype. The workspace holds
+ * the parts of rows whose keys are split over workgroups: jk_attn_q8_workspace_bytes(c, a) bytes (possibly
+ * 0, then it may be NULL), 16-byte aligned, of any content; calls that share one must not overlap. */
+size_t jk_attn_q8_workspace_bytes(const jk_kv_q8 *c, const jk_attn_q8_args *a);
+jk_status jk_attn_q8(jk_stream s, const jk_kv_q8 *c, const jk_attn_q8_args *a, void *workspace,
+                     size_t workspace_bytes);
+
+/* One step of beam search over `groups` groups of `width` hypotheses. The total of token t after hypothesis b is
+ * score_b + (x_bt - m_b - log(sum_u exp(x_bu - m_b))), m_b the row's largest logit; NaN logits count as -inf and a
+ * total that is NaN as -inf. A finished hypothesis (done != 0) goes on only as itself: token eos, its score as it is. The
+ * width best come out in order: larger total first, at equal totals the lower hypothesis, within one the larger
+ * logit, at equal logits the lower token. */
+typedef struct jk_beam_args {
+    const void *logits; /* [groups * width][vocab] */
+    int32_t dtype;
+    size_t groups, width, vocab; /* 1..65536, 1..32, 1..2^20 */
+    size_t stride;               /* elements from row to row; 0: vocab */
+    const float *scores;         /* [groups][width] */
+    const int32_t *done;         /* [groups][width], or NULL: none is */
+    int32_t eos;                 /* the token that finishes a hypothesis; -1: none (and done must be NULL) */
+    float *scores_out;           /* [groups][width] */
+    int32_t *parents, *tokens;   /* [groups][width]: hypothesis 0..width-1 of the group, token */
+    int32_t *done_out;           /* [groups][width]: parent done, or the token is eos; may be NULL */
+} jk_beam_args;
+/* The workspace (16-byte aligned, any content) holds each row's parts; calls that share one must not overlap.
+ * Outputs must not be arrays that the call reads. */
+size_t jk_beam_workspace_bytes(const jk_beam_args *a);
+jk_status jk_beam_select(jk_stream s, const jk_beam_args *a, void *workspace, size_t workspace_bytes);
+
 /* ---------------------------------------------------------------- measurement */
 
 /* A plain streaming read of `bytes` (a non-zero multiple of 16, 16-byte aligned) of device

@@ -223,6 +223,72 @@ __device__ __forceinline__ float gated(float g, float u) {
     }
 }
 
+// ------------------------------------------------------------ activations of several types
+// Element types of the entry points that take a jk_dtype. bf16 is the high half of an f32: widening is
+// a shift, rounding is to nearest even, NaN kept a NaN.
+struct F32 {
+    typedef float raw;
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+struct F16 {
+    typedef _Float16 raw;
+    static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
+    static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
+};
+struct BF16 {
+    typedef uint16_t raw;
+    static __device__ __forceinline__ float up(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+    static __device__ __forceinline__ uint16_t down(float v) {
+        const uint32_t b = __float_as_uint(v);
+        return __builtin_isnan(v) ? (uint16_t)((b >> 16) | 0x40u) : (uint16_t)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
+    }
+};
+
+// N consecutive elements (N a multiple of 8) as f32; vec: p is 16-byte aligned.
+template <typename T, int N>
+__device__ __forceinline__ void load_up(const typename T::raw *p, bool vec, float *out) {
+    typedef typename T::raw raw;
+    if (vec) {
+        constexpr int per = 16 / (int)sizeof(raw);
+#pragma unroll
+        for (int i = 0; i < N / per; ++i) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(p + i * per);
+            raw e[per];
+            __builtin_memcpy(e, &v, 16);
+#pragma unroll
+            for (int j = 0; j < per; ++j) out[i * per + j] = T::up(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = T::up(p[j]);
+    }
+}
+
+// N f32 values (N a multiple of 8) rounded to consecutive elements; vec: p is 16-byte aligned.
+template <typename T, int N>
+__device__ __forceinline__ void store_down(typename T::raw *p, bool vec, const float *v) {
+    typedef typename T::raw raw;
+    if (vec) {
+        constexpr int per = 16 / (int)sizeof(raw);
+#pragma unroll
+        for (int i = 0; i < N / per; ++i) {
+            raw e[per];
+#pragma unroll
+            for (int j = 0; j < per; ++j) e[j] = T::down(v[i * per + j]);
+            u32x4 w;
+            __builtin_memcpy(&w, e, 16);
+            *reinterpret_cast<u32x4 *>(p + i * per) = w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) p[j] = T::down(v[j]);
+    }
+}
+
+// Tokens of the paged cache: page ids and slots come from device memory and are checked before use.
+__device__ __forceinline__ bool page_ok(int id, int n_pages) { return (unsigned)id < (unsigned)n_pages; }
+
 // ------------------------------------------------------------ argmax keys
 // argmax_f32_scalar (lib.rs:555-568) as a maximum over 64-bit keys: the high word orders the
 // values (sign-magnitude bits mapped to an unsigned order, -0.0 folded onto +0.0 because the

@@ -186,6 +186,11 @@ jk_status gemm_i8_check(const int8_t *a, size_t a_len, size_t m, const int8_t *b
                         size_t k, const int32_t *c, size_t c_len);
 jk_status dot_i8_check(const int8_t *a, size_t a_len, const int8_t *b, size_t b_len, const int32_t *out);
 
+// Argument checks of a layer's 8-bit attention cache, shared by the entry points that take one.
+jk_status kv_check(const char *what, const jk_kv_q8 *c);
+inline bool dtype_ok(int t) { return t == JK_F32 || t == JK_F16 || t == JK_BF16; }
+inline size_t dtype_bytes(int t) { return t == JK_F32 ? 4 : 2; }
+
 // Checks the last kernel launch on the current thread.
 jk_status check_launch(const char *what);
 long cu_count();  // compute units of the device

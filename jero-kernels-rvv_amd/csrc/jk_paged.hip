@@ -1,0 +1,519 @@
+// jk_paged.hip -- the pages of a batch's attention cache: which page and slot each token of a step
+// goes to, the free pages' stack, and the rows' reordering after a beam search step.
+//
+// Everything that decides (prefix sums over the requests, whether a step fits) runs in one workgroup, so
+// a step's plan is one short launch with no hand-over between workgroups; only the per-token and
+// per-column writing of larger steps is spread over a second launch. All indices that come from
+// device memory are checked before they are used.
+#include <algorithm>
+
+#include "jk_device.hpp"
+
+namespace jk {
+
+constexpr int kPagedThreads = 1024;  // requests a pass of the planning workgroup takes
+
+struct PagedDev {
+    int n_requests, max_pages, n_pages, page_shift;
+    int32_t *lens, *table, *owned, *free_pages, *n_free;
+};
+
+__device__ __forceinline__ int pages_of(int tokens, int shift) { return (int)(((long)tokens + (1 << shift) - 1) >> shift); }
+
+// Exclusive prefix sum over the workgroup of one value per thread (the low and high words of v
+// are summed apart: the callers' sums stay below 2^31). *total gets the sum. s: 17 words of LDS.
+__device__ __forceinline__ unsigned long long wg_scan(unsigned long long v, unsigned long long *s,
+                                                      unsigned long long *total) {
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    unsigned long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long t = __shfl_up(inc, o, 64);
+        if (l >= o) inc += t;
+    }
+    __syncthreads();
+    if (l == 63) s[w] = inc;
+    __syncthreads();
+    unsigned long long base = 0, sum = 0;
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) {
+        if (i < w) base += s[i];
+        sum += s[i];
+    }
+    *total = sum;
+    return base + inc - v;
+}
+
+__device__ __forceinline__ long wg_sum(long v, long *s) {
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if (l == 0) s[w] = v;
+    __syncthreads();
+    long sum = 0;
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) sum += s[i];
+    return sum;
+}
+
+// Largest r with start[r] <= t among start[0..n) (start[0] <= t).
+template <typename P>
+__device__ __forceinline__ int owner_of(const P *start, int n, int t) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((int)start[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+struct StepDev {
+    int max_tokens;
+    int32_t *q_start, *slots, *positions, *requests, *status;
+};
+
+__device__ __forceinline__ void write_token(const StepDev &st, int t, int slot, int pos, int r) {
+    st.slots[t] = slot;
+    st.positions[t] = pos;
+    st.requests[t] = r;
+}
+
+// The plan of a step. FILL: this launch also numbers the tokens (few of them: one launch for a decode step).
+template <bool FILL>
+__global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p, const int32_t *__restrict__ n_new,
+                                                                     StepDev st, int32_t *lens_out,
+                                                                     int32_t *n_free_out) {
+    __shared__ unsigned long long s_scan[17];
+    __shared__ long s_sum[17];
+    __shared__ int s_tok[kPagedThreads + 1], s_pg[kPagedThreads + 1], s_len[kPagedThreads];
+    const int tid = threadIdx.x, page = 1 << p.page_shift;
+    const long cap = (long)p.max_pages << p.page_shift;
+    const int n_free = *p.n_free;
+
+    // does the step fit? (totals in 64 bits: counts are not trusted yet)
+    long tokens = 0, pages = 0, bad = (n_free < 0 || n_free > p.n_pages), over = 0;
+    for (int r = tid; r < p.n_requests; r += kPagedThreads) {
+        const long len = p.lens[r], n = n_new[r];
+        if (len < 0 || n < 0 || len > cap) {
+            bad = 1;
+            continue;
+        }
+        if (len + n > cap) over = 1;
+        tokens += n;
+        pages += ((len + n + page - 1) >> p.page_shift) - ((len + page - 1) >> p.page_shift);
+    }
+    tokens = wg_sum(tokens, s_sum);
+    pages = wg_sum(pages, s_sum);
+    const long flags = wg_sum(bad | (over << 32), s_sum);
+    const int status = (flags & 0xFFFFFFFFl) ? JK_PAGED_BAD_LENGTH
+                       : (flags >> 32) || tokens > st.max_tokens ? JK_PAGED_TOO_LONG
+                       : pages > n_free                          ? JK_PAGED_NO_PAGES
+                                                                 : JK_PAGED_OK;
+    if (tid == 0) {
+        *st.status = status;
+        *n_free_out = status == JK_PAGED_OK ? n_free - (int)pages : n_free;
+    }
+    if (status != JK_PAGED_OK) {
+        for (int r = tid; r < p.n_requests; r += kPagedThreads) {
+            st.q_start[r] = 0;
+            if (lens_out != p.lens) lens_out[r] = p.lens[r];
+        }
+        if (tid == 0) st.q_start[p.n_requests] = 0;
+        if constexpr (FILL)
+            for (int t = tid; t < st.max_tokens; t += kPagedThreads) write_token(st, t, -1, -1, -1);
+        return;
+    }
+
+    unsigned long long carry = 0;  // tokens (low word) and pages (high word) of the requests before this pass
+    for (int r0 = 0; r0 < p.n_requests; r0 += kPagedThreads) {
+        const int r = r0 + tid, nr = min(kPagedThreads, p.n_requests - r0);
+        const int len = r < p.n_requests ? p.lens[r] : 0, n = r < p.n_requests ? n_new[r] : 0;
+        const int more = pages_of(len + n, p.page_shift) - pages_of(len, p.page_shift);
+        unsigned long long sum;
+        const unsigned long long at = carry + wg_scan((unsigned long long)n | ((unsigned long long)more << 32),
+                                                      s_scan, &sum);
+        s_tok[tid] = (int)(uint32_t)at;
+        s_pg[tid] = (int)(at >> 32);
+        s_len[tid] = len;
+        if (r < p.n_requests) st.q_start[r] = (int)(uint32_t)at;
+        carry += sum;
+        if (tid == 0) {
+            s_tok[nr] = (int)(uint32_t)carry;
+            s_pg[nr] = (int)(carry >> 32);
+        }
+        __syncthreads();
+        if (r < p.n_requests) lens_out[r] = len + n;
+        // new pages, one a thread: entry m is page m - s_pg of its request, from the top of the stack down
+        for (int m = s_pg[0] + tid; m < s_pg[nr]; m += kPagedThreads) {
+            const int i = owner_of(s_pg, nr, m);
+            const int j = pages_of(s_len[i], p.page_shift) + m - s_pg[i];
+            const int id = p.free_pages[n_free - 1 - m];
+            const size_t cell = (size_t)(r0 + i) * p.max_pages + j;
+            p.table[cell] = p.owned[cell] = page_ok(id, p.n_pages) ? id : -1;
+        }
+        if constexpr (FILL) {
+            for (int t = s_tok[0] + tid; t < s_tok[nr]; t += kPagedThreads) {
+                const int i = owner_of(s_tok, nr, t), held = pages_of(s_len[i], p.page_shift);
+                const int pos = s_len[i] + t - s_tok[i], j = pos >> p.page_shift;
+                const int id = j < held ? p.table[(size_t)(r0 + i) * p.max_pages + j]
+                                        : p.free_pages[n_free - 1 - (s_pg[i] + j - held)];
+                write_token(st, t, page_ok(id, p.n_pages) ? (id << p.page_shift) + (pos & (page - 1)) : -1, pos,
+                            r0 + i);
+            }
+        }
+        __syncthreads();
+    }
+    const int total = (int)(uint32_t)carry;
+    if (tid == 0) st.q_start[p.n_requests] = total;
+    if constexpr (FILL)
+        for (int t = total + tid; t < st.max_tokens; t += kPagedThreads) write_token(st, t, -1, -1, -1);
+}
+
+// Numbers the tokens of a planned step from q_start, the new lengths and the table.
+constexpr int kFillThreads = 256;
+__global__ __launch_bounds__(kFillThreads) void paged_fill_kernel(PagedDev p, StepDev st,
+                                                                  const int32_t *__restrict__ lens) {
+    __shared__ int s_start[kPagedThreads + 1];
+    const bool staged = p.n_requests <= kPagedThreads;
+    if (staged)
+        for (int i = threadIdx.x; i <= p.n_requests; i += kFillThreads) s_start[i] = st.q_start[i];
+    __syncthreads();
+    const int t = blockIdx.x * kFillThreads + threadIdx.x;
+    if (t >= st.max_tokens) return;
+    if (t >= (staged ? s_start[p.n_requests] : st.q_start[p.n_requests])) return write_token(st, t, -1, -1, -1);
+    const int r = staged ? owner_of(s_start, p.n_requests, t) : owner_of(st.q_start, p.n_requests, t);
+    const int end = staged ? s_start[r + 1] : st.q_start[r + 1];
+    const int pos = lens[r] - (end - t);
+    const int id = p.table[(size_t)r * p.max_pages + (pos >> p.page_shift)];
+    write_token(st, t, page_ok(id, p.n_pages) ? (id << p.page_shift) + (pos & ((1 << p.page_shift) - 1)) : -1, pos, r);
+}
+
+__global__ __launch_bounds__(256) void paged_reset_kernel(PagedDev p) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, cells = (size_t)p.n_requests * p.max_pages;
+    if (i < cells) p.table[i] = p.owned[i] = -1;
+    if (i < (size_t)p.n_requests) p.lens[i] = 0;
+    if (i < (size_t)p.n_pages) p.free_pages[i] = p.n_pages - 1 - (int)i;
+    if (i == 0) *p.n_free = p.n_pages;
+}
+
+// One workgroup. Each wave counts the owned pages of its requests, a prefix sum places them, and the wave
+// writes them in order of their places.
+__global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p, const int32_t *__restrict__ ended) {
+    __shared__ unsigned long long s_scan[17];
+    __shared__ int s_cnt[kPagedThreads];
+    const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+    long height = min(max(*p.n_free, 0), p.n_pages);
+    for (int r0 = 0; r0 < p.n_requests; r0 += kPagedThreads) {
+        const int nr = min(kPagedThreads, p.n_requests - r0);
+        for (int i = w; i < nr; i += kPagedThreads / 64) {
+            int n = 0;
+            if (ended[r0 + i])
+                for (int j = l; j < p.max_pages; j += 64)
+                    n += page_ok(p.owned[(size_t)(r0 + i) * p.max_pages + j], p.n_pages);
+            n = wave_sum64_dpp(n);
+            if (l == 0) s_cnt[i] = n;
+        }
+        __syncthreads();
+        const int mine = tid < nr ? s_cnt[tid] : 0;
+        unsigned long long sum;
+        const int before = (int)wg_scan((unsigned long long)mine, s_scan, &sum);
+        __syncthreads();
+        if (tid < nr) s_cnt[tid] = before;
+        __syncthreads();
+        for (int i = w; i < nr; i += kPagedThreads / 64) {
+            if (!ended[r0 + i]) continue;
+            long at = height + s_cnt[i];
+            for (int j0 = 0; j0 < p.max_pages; j0 += 64) {
+                const int j = j0 + l;
+                const size_t cell = (size_t)(r0 + i) * p.max_pages + j;
+                const int id = j < p.max_pages ? p.owned[cell] : -1;
+                const unsigned long long has = __ballot(page_ok(id, p.n_pages));
+                const long to = at + __popcll(has & ((1ull << l) - 1));
+                if (page_ok(id, p.n_pages) && to < p.n_pages) p.free_pages[to] = id;
+                if (j < p.max_pages) p.owned[cell] = p.table[cell] = -1;
+                at += __popcll(has);
+            }
+            if (l == 0) p.lens[r0 + i] = 0;
+        }
+        height += (long)sum;
+        __syncthreads();
+    }
+    if (tid == 0) *p.n_free = (int)min(height, (long)p.n_pages);
+}
+
+// The row that row r of a group goes on from.
+__device__ __forceinline__ int parent_row(const int32_t *parent, int row, int width) {
+    const int b = row % width, q = parent[row];
+    return (unsigned)q < (unsigned)width ? row - b + q : row;
+}
+
+// First half of the reordering, in one workgroup: takes a page for each row that has none to go on
+// filling, and writes the new lengths. Passes hold whole groups, so that in place a group's lengths are
+// all read before one of them is written.
+__global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(PagedDev p,
+                                                                           const int32_t *__restrict__ parent,
+                                                                           int width, int32_t *status,
+                                                                           int32_t *lens_out) {
+    __shared__ unsigned long long s_scan[17];
+    __shared__ long s_sum[17];
+    const int tid = threadIdx.x, mask = (1 << p.page_shift) - 1;
+    const long cap = (long)p.max_pages << p.page_shift;
+    const int n_free = *p.n_free, per = kPagedThreads / width * width;
+    // needs(row): whether it takes a page; flags get what is wrong with its parent
+    auto look = [&](int row, int *len, long *flags) -> bool {
+        const int from = parent_row(parent, row, width);
+        *len = p.lens[from];
+        if (*len < 0 || *len > cap) {
+            *flags |= 1;
+            return false;
+        }
+        if ((*len & mask) == 0) return false;
+        const int j = *len >> p.page_shift;
+        const int own = p.owned[(size_t)from * p.max_pages + j];
+        if (!page_ok(own, p.n_pages) || own != p.table[(size_t)from * p.max_pages + j]) *flags |= 1l << 32;
+        return !page_ok(p.owned[(size_t)row * p.max_pages + j], p.n_pages);
+    };
+    long need = 0, flags = 0;
+    int len;
+    for (int row = tid; row < p.n_requests; row += kPagedThreads) {
+        long f = 0;
+        need += look(row, &len, &f);
+        flags |= f;
+    }
+    need = wg_sum(need, s_sum);
+    flags = wg_sum(flags, s_sum);
+    const int st = (flags & 0xFFFFFFFFl) || n_free < 0 || n_free > p.n_pages ? JK_PAGED_BAD_LENGTH
+                   : flags                                                  ? JK_PAGED_NOT_OWNED
+                   : need > n_free                                          ? JK_PAGED_NO_PAGES
+                                                                            : JK_PAGED_OK;
+    __syncthreads();  // (every thread has read n_free)
+    if (tid == 0) {
+        *status = st;
+        if (st == JK_PAGED_OK) *p.n_free = n_free - (int)need;
+    }
+    if (st != JK_PAGED_OK) {
+        if (lens_out != p.lens)
+            for (int row = tid; row < p.n_requests; row += kPagedThreads) lens_out[row] = p.lens[row];
+        return;
+    }
+    int taken = 0;
+    for (int r0 = 0; r0 < p.n_requests; r0 += per) {
+        const int row = r0 + tid;
+        const bool live = tid < per && row < p.n_requests;
+        bool takes = false;
+        long f = 0;
+        len = 0;
+        if (live) takes = look(row, &len, &f);
+        unsigned long long sum;
+        const int at = taken + (int)wg_scan((unsigned long long)takes, s_scan, &sum);  // (a barrier: all have read)
+        if (takes) {
+            const int id = p.free_pages[n_free - 1 - at];
+            p.owned[(size_t)row * p.max_pages + (len >> p.page_shift)] = page_ok(id, p.n_pages) ? id : -1;
+        }
+        if (live) lens_out[row] = len;
+        taken += (int)sum;
+    }
+}
+
+// Second half: one thread takes one column of a group's rows, reads all of them and then writes them, so the
+// permutation can be in place. lens: the new lengths.
+template <int MW>
+__global__ __launch_bounds__(256) void paged_reorder_table_kernel(PagedDev p, const int32_t *__restrict__ parent,
+                                                                  int width, const int32_t *__restrict__ status,
+                                                                  const int32_t *__restrict__ lens, int32_t *table_out,
+                                                                  int col_blocks) {
+    const int g = blockIdx.x / col_blocks, j = (blockIdx.x % col_blocks) * 256 + threadIdx.x;
+    if (j >= p.max_pages) return;
+    const int row0 = g * width, mask = (1 << p.page_shift) - 1;
+    const bool ok = *status == JK_PAGED_OK;
+    if (!ok && table_out == p.table) return;
+    int v[MW];
+#pragma unroll
+    for (int b = 0; b < MW; ++b) {
+        if (b >= width) break;
+        const int row = row0 + b, len = lens[row], full = len >> p.page_shift;
+        if (!ok) v[b] = p.table[(size_t)row * p.max_pages + j];
+        else if (j < full) v[b] = p.table[(size_t)parent_row(parent, row, width) * p.max_pages + j];
+        else v[b] = j == full && (len & mask) ? p.owned[(size_t)row * p.max_pages + j] : -1;
+    }
+#pragma unroll
+    for (int b = 0; b < MW; ++b) {
+        if (b >= width) break;
+        table_out[(size_t)(row0 + b) * p.max_pages + j] = v[b];
+    }
+}
+
+// Moves the pages that are being filled: one thread takes 16 bytes of one head's rows of every
+// hypothesis of a group, reads all of them and then writes them (a page can be read by one row and
+// overwritten by another's in the same step).
+template <int MW>
+__global__ __launch_bounds__(256) void kv_reorder_kernel(PagedDev p, jk_kv_q8 c, const int32_t *__restrict__ parent,
+                                                         int width, const int32_t *__restrict__ status, int blocks) {
+    if (*status != JK_PAGED_OK) return;
+    const int cell = blockIdx.x / blocks, i = (blockIdx.x % blocks) * 256 + threadIdx.x;
+    const int heads = (int)c.n_kv, which = cell % 2, h = cell / 2 % heads, row0 = cell / 2 / heads * width;
+    int8_t *codes = which ? c.v : c.k;
+    float *scales = which ? c.v_scale : c.k_scale;
+    const int mask = (1 << p.page_shift) - 1, hd = (int)c.head_dim;
+    const long cap = (long)p.max_pages << p.page_shift;
+    u32x4 v[MW];
+    float sc[MW];
+    bool moves[MW];
+    size_t to[MW];
+#pragma unroll
+    for (int b = 0; b < MW; ++b) {
+        moves[b] = false;
+        if (b >= width) continue;
+        const int row = row0 + b, from = parent_row(parent, row, width), len = p.lens[row];
+        if (from == row || len <= 0 || len > cap || (len & mask) == 0) continue;
+        const int j = len >> p.page_shift;
+        const int src = p.owned[(size_t)from * p.max_pages + j], dst = p.owned[(size_t)row * p.max_pages + j];
+        if (!page_ok(src, p.n_pages) || !page_ok(dst, p.n_pages) || i * 16 >= (len & mask) * hd) continue;
+        moves[b] = true;
+        const size_t from_head = (size_t)src * heads + h;
+        to[b] = (size_t)dst * heads + h;
+        v[b] = *reinterpret_cast<const u32x4 *>(codes + (from_head << p.page_shift) * hd + (size_t)i * 16);
+        sc[b] = i == 0 ? scales[from_head] : 0.0f;  // (a head's scales are one thread's to read and write)
+    }
+#pragma unroll
+    for (int b = 0; b < MW; ++b) {
+        if (!moves[b]) continue;
+        *reinterpret_cast<u32x4 *>(codes + (to[b] << p.page_shift) * hd + (size_t)i * 16) = v[b];
+        if (i == 0) scales[to[b]] = sc[b];
+    }
+}
+
+constexpr size_t kMaxBlocks = ((size_t)1 << 24) - 1;  // of 256 threads in one launch
+
+static int log2_of(size_t v) {
+    int s = 0;
+    while (((size_t)1 << s) < v) ++s;
+    return s;
+}
+
+static jk_status paged_check(const char *what, const jk_paged *p, PagedDev *out) {
+    if (!p) return fail(JK_TENSOR_BOUNDS, "%s: null jk_paged", what);
+    if (!p->lens || !p->table || !p->owned || !p->free_pages || !p->n_free)
+        return fail(JK_TENSOR_BOUNDS, "%s: null array in jk_paged", what);
+    if (p->page < 16 || p->page > 256 || (p->page & (p->page - 1)))
+        return fail(JK_TENSOR_BOUNDS, "%s: %zu tokens a page: 16, 32, 64, 128 or 256", what, p->page);
+    if (p->n_requests == 0 || p->max_pages == 0 || p->n_pages == 0)
+        return fail(JK_TENSOR_BOUNDS, "%s: no requests, columns or pages", what);
+    if (p->n_requests > (size_t)INT32_MAX / 64 || p->max_pages > (size_t)INT32_MAX / p->page ||
+        p->n_pages > (size_t)INT32_MAX / p->page)
+        return fail(JK_TENSOR_BOUNDS, "%s: %zu requests, %zu columns or %zu pages of %zu tokens exceed the int32 range",
+                    what, p->n_requests, p->max_pages, p->n_pages, p->page);
+    *out = PagedDev{(int)p->n_requests, (int)p->max_pages, (int)p->n_pages, log2_of(p->page),
+                    p->lens,            p->table,          p->owned,        p->free_pages,
+                    p->n_free};
+    return JK_OK;
+}
+
+static jk_status width_check(const char *what, const jk_paged *p, size_t width) {
+    if (width == 0 || width > 32 || p->n_requests % width)
+        return fail(JK_TENSOR_BOUNDS, "%s: width %zu: 1..32, and %zu requests a multiple of it", what, width,
+                    p->n_requests);
+    if (p->owned == p->table)
+        return fail(JK_TENSOR_BOUNDS, "%s: owned and table are the same array: rows that share pages need both", what);
+    return JK_OK;
+}
+
+}  // namespace jk
+
+using namespace jk;
+
+extern "C" {
+
+jk_status jk_paged_reset(jk_stream s, const jk_paged *p) {
+    PagedDev d;
+    JK_TRY(paged_check("paged_reset", p, &d));
+    const size_t cells = std::max({p->n_requests * p->max_pages, p->n_requests, p->n_pages});
+    if (cells > (size_t)INT32_MAX)
+        return fail(JK_TENSOR_BOUNDS, "paged_reset: a table of %zu x %zu is too large", p->n_requests, p->max_pages);
+    hipLaunchKernelGGL(paged_reset_kernel, dim3((unsigned)((cells + 255) / 256)), dim3(256), 0, (hipStream_t)s, d);
+    return check_launch("paged_reset_kernel");
+}
+
+jk_status jk_paged_extend(jk_stream s, const jk_paged *p, const int32_t *n_new, const jk_paged_step *st,
+                          int32_t *lens_out, int32_t *n_free_out) {
+    PagedDev d;
+    JK_TRY(paged_check("paged_extend", p, &d));
+    if (!n_new || !st || !st->q_start || !st->status)
+        return fail(JK_TENSOR_BOUNDS, "paged_extend: null counts, step, q_start or status");
+    if (st->max_tokens && (!st->slots || !st->positions || !st->requests))
+        return fail(JK_TENSOR_BOUNDS, "paged_extend: null slots, positions or requests");
+    if (st->max_tokens > (size_t)INT32_MAX - 1024)
+        return fail(JK_TENSOR_BOUNDS, "paged_extend: %zu tokens exceed the int32 range", st->max_tokens);
+    const StepDev sd{(int)st->max_tokens, st->q_start, st->slots, st->positions, st->requests, st->status};
+    int32_t *lo = lens_out ? lens_out : p->lens, *fo = n_free_out ? n_free_out : p->n_free;
+    // one workgroup numbers up to this many tokens itself
+    if (st->max_tokens <= 2 * kPagedThreads) {
+        hipLaunchKernelGGL(paged_extend_kernel<true>, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, n_new, sd, lo,
+                           fo);
+        return check_launch("paged_extend_kernel");
+    }
+    hipLaunchKernelGGL(paged_extend_kernel<false>, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, n_new, sd, lo, fo);
+    JK_TRY(check_launch("paged_extend_kernel"));
+    hipLaunchKernelGGL(paged_fill_kernel, dim3((unsigned)((st->max_tokens + kFillThreads - 1) / kFillThreads)),
+                       dim3(kFillThreads), 0, (hipStream_t)s, d, sd, lo);
+    return check_launch("paged_fill_kernel");
+}
+
+jk_status jk_paged_release(jk_stream s, const jk_paged *p, const int32_t *ended) {
+    PagedDev d;
+    JK_TRY(paged_check("paged_release", p, &d));
+    if (!ended) return fail(JK_TENSOR_BOUNDS, "paged_release: null flags");
+    hipLaunchKernelGGL(paged_release_kernel, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, ended);
+    return check_launch("paged_release_kernel");
+}
+
+jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent, size_t width, int32_t *status,
+                           int32_t *lens_out, int32_t *table_out) {
+    PagedDev d;
+    JK_TRY(paged_check("paged_reorder", p, &d));
+    JK_TRY(width_check("paged_reorder", p, width));
+    if (!parent || !status) return fail(JK_TENSOR_BOUNDS, "paged_reorder: null parents or status");
+    if (!lens_out != !table_out)
+        return fail(JK_TENSOR_BOUNDS, "paged_reorder: lens_out and table_out are given both or neither");
+    if (table_out == p->owned) return fail(JK_TENSOR_BOUNDS, "paged_reorder: table_out is owned");
+    int32_t *lo = lens_out ? lens_out : p->lens, *to = table_out ? table_out : p->table;
+    const size_t col_blocks = (p->max_pages + 255) / 256, groups = p->n_requests / width;
+    if (col_blocks * groups > kMaxBlocks)
+        return fail(JK_TENSOR_BOUNDS, "paged_reorder: a table of %zu x %zu is too large", p->n_requests, p->max_pages);
+    hipLaunchKernelGGL(paged_reorder_plan_kernel, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, parent, (int)width,
+                       status, lo);
+    JK_TRY(check_launch("paged_reorder_plan_kernel"));
+    const dim3 grid((unsigned)(col_blocks * groups));
+    if (width <= 8)
+        hipLaunchKernelGGL(paged_reorder_table_kernel<8>, grid, dim3(256), 0, (hipStream_t)s, d, parent, (int)width,
+                           status, lo, to, (int)col_blocks);
+    else
+        hipLaunchKernelGGL(paged_reorder_table_kernel<32>, grid, dim3(256), 0, (hipStream_t)s, d, parent, (int)width,
+                           status, lo, to, (int)col_blocks);
+    return check_launch("paged_reorder_table_kernel");
+}
+
+jk_status jk_kv_reorder_q8(jk_stream s, const jk_kv_q8 *c, const jk_paged *p, const int32_t *parent, size_t width,
+                           const int32_t *status) {
+    PagedDev d;
+    JK_TRY(kv_check("kv_reorder_q8", c));
+    JK_TRY(paged_check("kv_reorder_q8", p, &d));
+    JK_TRY(width_check("kv_reorder_q8", p, width));
+    if (c->page != p->page || c->n_pages != p->n_pages)
+        return fail(JK_TENSOR_BOUNDS, "kv_reorder_q8: a cache of %zu pages of %zu tokens for tables of %zu of %zu",
+                    c->n_pages, c->page, p->n_pages, p->page);
+    if (!parent || !status) return fail(JK_TENSOR_BOUNDS, "kv_reorder_q8: null parents or status");
+    const size_t blocks = (c->page * c->head_dim / 16 + 255) / 256, cells = p->n_requests / width * c->n_kv * 2;
+    if (cells * blocks > kMaxBlocks)
+        return fail(JK_TENSOR_BOUNDS, "kv_reorder_q8: %zu requests of %zu heads are too many", p->n_requests, c->n_kv);
+    const dim3 grid((unsigned)(cells * blocks));
+    if (width <= 8)
+        hipLaunchKernelGGL(kv_reorder_kernel<8>, grid, dim3(256), 0, (hipStream_t)s, d, *c, parent, (int)width, status,
+                           (int)blocks);
+    else
+        hipLaunchKernelGGL(kv_reorder_kernel<32>, grid, dim3(256), 0, (hipStream_t)s, d, *c, parent, (int)width, status,
+                           (int)blocks);
+    return check_launch("kv_reorder_kernel");
+}
+
+}  // extern "C"

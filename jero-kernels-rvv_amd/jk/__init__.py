@@ -135,6 +135,8 @@ def lib() -> C.CDLL:
         h = C.CDLL(LIB_PATH)
         h.jk_last_error.restype = C.c_char_p
         h.jk_act_q8_bytes.restype = _sz
+        h.jk_attn_q8_workspace_bytes.restype = _sz
+        h.jk_beam_workspace_bytes.restype = _sz
         h.jk_act_q8_bytes.argtypes = [_sz, _sz]
         _lib_handle = h
     return _lib_handle
@@ -803,6 +805,199 @@ def op_counts() -> tuple[int, int]:
     t, v = C.c_uint64(0), C.c_uint64(0)
     lib().jk_op_counts(C.byref(t), C.byref(v))
     return t.value, v.value
+
+
+# ------------------------------------------- paged 8-bit attention cache, beam search
+F32, F16, BF16 = 0, 1, 30  # jk_dtype
+PAGED_OK, PAGED_NO_PAGES, PAGED_TOO_LONG, PAGED_BAD_LENGTH, PAGED_NOT_OWNED = 0, 1, 2, 3, 4
+_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "float32": F32, "float16": F16}
+
+
+class PagedC(C.Structure):
+    _fields_ = [("n_requests", _sz), ("max_pages", _sz), ("n_pages", _sz), ("page", _sz), ("lens", _vp),
+                ("table", _vp), ("owned", _vp), ("free_pages", _vp), ("n_free", _vp)]
+
+
+class PagedStepC(C.Structure):
+    _fields_ = [("max_tokens", _sz), ("q_start", _vp), ("slots", _vp), ("positions", _vp), ("requests", _vp),
+                ("status", _vp)]
+
+
+class KvQ8C(C.Structure):
+    _fields_ = [("n_pages", _sz), ("page", _sz), ("n_kv", _sz), ("head_dim", _sz), ("k", _vp), ("v", _vp),
+                ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class AttnQ8ArgsC(C.Structure):
+    _fields_ = [("q", _vp), ("out", _vp), ("dtype", C.c_int32), ("n_tokens", _sz), ("n_heads", _sz),
+                ("q_stride_token", _sz), ("q_stride_head", _sz), ("out_stride_token", _sz), ("out_stride_head", _sz),
+                ("n_requests", _sz), ("max_pages", _sz), ("q_start", _vp), ("lens", _vp), ("table", _vp),
+                ("max_new", _sz), ("max_len", _sz), ("scale", C.c_float), ("window", _sz)]
+
+
+class BeamArgsC(C.Structure):
+    _fields_ = [("logits", _vp), ("dtype", C.c_int32), ("groups", _sz), ("width", _sz), ("vocab", _sz),
+                ("stride", _sz), ("scores", _vp), ("done", _vp), ("eos", C.c_int32), ("scores_out", _vp),
+                ("parents", _vp), ("tokens", _vp), ("done_out", _vp)]
+
+
+def _dtype_of(x) -> int:
+    t = _DTYPES.get(str(x.dtype))
+    if t is None:
+        raise CapabilityMismatch(f"element type {x.dtype}: float32, float16 or bfloat16")
+    return t
+
+
+def _strides(x) -> tuple[int, int]:
+    """Token and head strides of a [tokens][heads][head_dim] tensor whose last dimension is packed."""
+    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise TensorBoundsError("a [tokens][heads][head_dim] tensor with a packed last dimension is needed")
+    return x.stride(0), x.stride(1)
+
+
+def _held(struct, *tensors):
+    """The struct, which keeps the tensors whose addresses it holds."""
+    struct.tensors = tensors
+    return struct
+
+
+def _i32(*tensors):
+    for x in tensors:
+        if x is not None and (str(x.dtype) != "torch.int32" or not x.is_contiguous()):
+            raise TensorBoundsError("a packed int32 tensor is needed")
+
+
+def paged(lens, table, owned, free_pages, n_free, page: int) -> PagedC:
+    """jk_paged of int32 device tensors: lens [requests], table and owned [requests][columns], free_pages
+    [pages], n_free [1]."""
+    _i32(lens, table, owned, free_pages, n_free)
+    if table.shape != owned.shape or table.dim() != 2 or table.shape[0] != lens.numel():
+        raise TensorBoundsError("table and owned need one row a request and the same columns")
+    return _held(PagedC(lens.numel(), table.shape[1], free_pages.numel(), page, _ptr(lens), _ptr(table), _ptr(owned),
+                        _ptr(free_pages), _ptr(n_free)), lens, table, owned, free_pages, n_free)
+
+
+def paged_step(q_start, slots, positions, requests, status) -> PagedStepC:
+    """jk_paged_step of int32 device tensors: q_start [requests + 1], the others [tokens], status [1]."""
+    _i32(q_start, slots, positions, requests, status)
+    if not slots.numel() == positions.numel() == requests.numel():
+        raise TensorBoundsError("slots, positions and requests need the same length")
+    return _held(PagedStepC(slots.numel(), _ptr(q_start), _ptr(slots), _ptr(positions), _ptr(requests), _ptr(status)),
+                 q_start, slots, positions, requests, status)
+
+
+def dev_paged_reset(p: PagedC, stream=None):
+    """jk_paged_reset: empty requests, all pages free."""
+    _check(lib().jk_paged_reset(_vp(stream or 0), C.byref(p)))
+
+
+def dev_paged_extend(p: PagedC, n_new, step: PagedStepC, lens_out=None, n_free_out=None, stream=None):
+    """jk_paged_extend: n_new[r] more tokens for each request; pages, slots and positions of the step's tokens."""
+    _check(lib().jk_paged_extend(_vp(stream or 0), C.byref(p), _vp(_ptr(n_new)), C.byref(step), _vp(_ptr(lens_out)),
+                                 _vp(_ptr(n_free_out))))
+
+
+def dev_paged_release(p: PagedC, ended, stream=None):
+    """jk_paged_release: the pages of the requests with ended[r] != 0 back on the stack."""
+    _check(lib().jk_paged_release(_vp(stream or 0), C.byref(p), _vp(_ptr(ended))))
+
+
+def dev_paged_reorder(p: PagedC, parent, width: int, status, lens_out=None, table_out=None, stream=None):
+    """jk_paged_reorder: row r of each group of `width` goes on from row parent[r]."""
+    _check(lib().jk_paged_reorder(_vp(stream or 0), C.byref(p), _vp(_ptr(parent)), _sz(width), _vp(_ptr(status)),
+                                  _vp(_ptr(lens_out)), _vp(_ptr(table_out))))
+
+
+def kv_q8(k, v, k_scale, v_scale) -> KvQ8C:
+    """jk_kv_q8 of device tensors: int8 k and v [pages][kv heads][page][head_dim], f32 scales [pages][kv heads]."""
+    for c, sc in ((k, k_scale), (v, v_scale)):
+        if str(c.dtype) != "torch.int8" or c.dim() != 4 or not c.is_contiguous() or c.shape != k.shape:
+            raise TensorBoundsError("codes need packed int8 tensors [pages][kv heads][page][head_dim]")
+        if str(sc.dtype) != "torch.float32" or not sc.is_contiguous() or tuple(sc.shape) != tuple(c.shape[:2]):
+            raise TensorBoundsError("scales need packed float32 tensors [pages][kv heads]")
+    n, kv, page, hd = k.shape
+    return _held(KvQ8C(n, page, kv, hd, _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale)), k, v, k_scale, v_scale)
+
+
+def dev_kv_append_q8(c: KvQ8C, k, v, slots, stream=None):
+    """jk_kv_append_q8: k and v [tokens][kv heads][head_dim] (the same strides) into their slots."""
+    st, sh = _strides(k)
+    if _strides(v) != (st, sh) or v.shape != k.shape or v.dtype != k.dtype:
+        raise TensorBoundsError("keys and values need the same shape, strides and type")
+    if tuple(k.shape[1:]) != (c.n_kv, c.head_dim) or slots.numel() != k.shape[0]:
+        raise TensorBoundsError("keys of the cache's heads and one slot a token are needed")
+    _i32(slots)
+    _check(lib().jk_kv_append_q8(_vp(stream or 0), C.byref(c), _vp(_ptr(k)), _vp(_ptr(v)), C.c_int(_dtype_of(k)),
+                                 _sz(k.shape[0]), _sz(st), _sz(sh), _vp(_ptr(slots))))
+
+
+def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
+    """jk_kv_read_q8: the values of the slots, packed [slots][kv heads][head_dim]; either output may be None."""
+    _i32(slots)
+    outs = [x for x in (k_out, v_out) if x is not None]
+    for x in outs:
+        if not x.is_contiguous() or x.numel() != slots.numel() * c.n_kv * c.head_dim or x.dtype != outs[0].dtype:
+            raise TensorBoundsError("outputs need packed tensors [slots][kv heads][head_dim] of one type")
+    _check(lib().jk_kv_read_q8(_vp(stream or 0), C.byref(c), _vp(_ptr(slots)), _sz(slots.numel()),
+                               C.c_int(_dtype_of(outs[0]) if outs else F32), _vp(_ptr(k_out)), _vp(_ptr(v_out))))
+
+
+def dev_kv_reorder_q8(c: KvQ8C, p: PagedC, parent, width: int, status, stream=None):
+    """jk_kv_reorder_q8: the cache's part of dev_paged_reorder, after it, for each layer."""
+    _check(lib().jk_kv_reorder_q8(_vp(stream or 0), C.byref(c), C.byref(p), _vp(_ptr(parent)), _sz(width),
+                                  _vp(_ptr(status))))
+
+
+def attn_q8_args(q, out, q_start, lens, table, max_new: int, max_len: int, scale: float, window: int = 0) -> AttnQ8ArgsC:
+    """jk_attn_q8_args of device tensors: q and out [tokens][heads][head_dim] of one type, int32 q_start
+    [requests + 1], lens [requests] and table [requests][columns]."""
+    (qt, qh), (ot, oh) = _strides(q), _strides(out)
+    _i32(q_start, lens, table)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise TensorBoundsError("queries and output need the same shape and type")
+    if table.dim() != 2 or table.shape[0] != lens.numel() or q_start.numel() != lens.numel() + 1:
+        raise TensorBoundsError("one length and one row of the table a request and one more q_start are needed")
+    return _held(AttnQ8ArgsC(_ptr(q), _ptr(out), _dtype_of(q), q.shape[0], q.shape[1], qt, qh, ot, oh, lens.numel(),
+                             table.shape[1], _ptr(q_start), _ptr(lens), _ptr(table), max_new, max_len, scale, window),
+                 q, out, q_start, lens, table)
+
+
+def attn_q8_workspace_bytes(c: KvQ8C, a: AttnQ8ArgsC) -> int:
+    """Device workspace bytes of dev_attn_q8 (may be 0)."""
+    return int(lib().jk_attn_q8_workspace_bytes(C.byref(c), C.byref(a)))
+
+
+def dev_attn_q8(c: KvQ8C, a: AttnQ8ArgsC, ws=None, stream=None, ws_bytes=None):
+    """jk_attn_q8: causal attention of the step's queries over the paged 8-bit cache."""
+    _check(lib().jk_attn_q8(_vp(stream or 0), C.byref(c), C.byref(a), _vp(_ptr(ws)), _sz(_ws_bytes(ws, ws_bytes))))
+
+
+def beam_args(logits, scores, done, scores_out, parents, tokens, done_out=None, eos: int = -1) -> BeamArgsC:
+    """jk_beam_args of device tensors: logits [groups * width][vocab] (rows may be strided), f32 scores and
+    scores_out and int32 done (or None), parents, tokens and done_out (or None) [groups][width]."""
+    _i32(done, parents, tokens, done_out)
+    groups, width = scores.shape
+    for x in (scores, done, scores_out, parents, tokens, done_out):
+        if x is not None and (tuple(x.shape) != (groups, width) or not x.is_contiguous()):
+            raise TensorBoundsError("scores, done, parents and tokens need packed tensors [groups][width]")
+    if str(scores.dtype) != "torch.float32" or str(scores_out.dtype) != "torch.float32":
+        raise TensorBoundsError("scores need float32 tensors")
+    if logits.dim() != 2 or logits.shape[0] != groups * width or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise TensorBoundsError("logits need one packed row a hypothesis")
+    stride = logits.stride(0) if logits.shape[0] > 1 else 0
+    return _held(BeamArgsC(_ptr(logits), _dtype_of(logits), groups, width, logits.shape[1], stride, _ptr(scores),
+                           _ptr(done), eos, _ptr(scores_out), _ptr(parents), _ptr(tokens), _ptr(done_out)),
+                 logits, scores, done, scores_out, parents, tokens, done_out)
+
+
+def beam_workspace_bytes(a: BeamArgsC) -> int:
+    """Device workspace bytes of dev_beam_select."""
+    return int(lib().jk_beam_workspace_bytes(C.byref(a)))
+
+
+def dev_beam_select(a: BeamArgsC, ws, stream=None, ws_bytes=None):
+    """jk_beam_select: the width best continuations of each group's hypotheses."""
+    _check(lib().jk_beam_select(_vp(stream or 0), C.byref(a), _vp(_ptr(ws)), _sz(_ws_bytes(ws, ws_bytes))))
 
 
 def dev_measure_stream_read(buf, nbytes, sink, stream=None):
