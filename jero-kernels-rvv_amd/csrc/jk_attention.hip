@@ -7,7 +7,7 @@
 //   s_j = scale q.k_j,  p_j = exp(s_j - m),  l = sum p_j,  o = sum p_j v_j / l
 // with k_j = ks * codes and v_j = vs * codes, ks and vs one number per page and head. The products run on f16
 // matrix instructions: codes are exact in f16, ks multiplies the finished score, and vs joins the
-// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j <= 1 whatever the values' size; o is
+// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j <= 1 whatever the values' size (held times 2^14); o is
 // rescaled by r like by m. Scores are computed transposed (rows = tokens), so a lane that holds a column's
 // scores of four consecutive tokens holds them just as the second product's operand wants them: the order
 // of the tokens inside a matrix instruction is free as long as both of its operands agree on it.
@@ -24,6 +24,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kCodeScale = 512.0f;  // a code becomes code / 512 in f16 (code_pair)
+// Queries and weights are held in f16 with their largest values near 2^14, so that what is 2^-28 of those is still a
+// normal number, and the low parts of f32 ones keep their bits: weights are p_j vs / r times this.
+constexpr float kWeightScale = 16384.0f;
 
 struct AttnDev {
     const void *q;
@@ -102,10 +105,38 @@ __device__ __forceinline__ f16x8 codes_across(const uint32_t *w, int b) {
     return u.v;
 }
 
+// Maximum over the four lanes of a column (lanes 16 apart).
+__device__ __forceinline__ float max_rows(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Eight f32 values as f16 (PARTS 1), or as two f16 that add up to 22 bits of them. The low part is taken from the very
+// number that the high part became: the empty asm keeps the compiler from converting y a second time with another
+// instruction, which was seen to round some values to the other neighbour.
+template <int PARTS>
+__device__ __forceinline__ void split_f16(const float *y, f16x8 *out) {
+    union {
+        f16x8 v;
+        uint32_t w[4];
+    } hi;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) hi.v[i] = (_Float16)y[i];
+    if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("" : "+v"(hi.w[i]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[1][i] = (_Float16)(y[i] - (float)hi.v[i]);
+    }
+    out[0] = hi.v;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Power of two that brings a row whose largest |value| is m to [0.5, 1) (zeros, infinities and NaN: any).
-__device__ __forceinline__ int down_shift(float m) { return 126 - (int)((__float_as_uint(m) >> 23) & 255u); }
+// Power of two that brings a row whose largest |value| is m to [2^13, 2^14) (zeros, infinities and NaN: any).
+__device__ __forceinline__ int range_shift(float m) { return 140 - (int)((__float_as_uint(m) >> 23) & 255u); }
 
 // Up to 16 columns of one request and kv head over one split of its keys, by four waves that take 32 tokens in
 // turn; their sums are joined in LDS. A lane (n = lane % 16, g = lane / 16) holds of column n: the query's
@@ -119,7 +150,7 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
     constexpr int KJ = HDP / 64, NT = HDP / 16, VW = HDP / 64;  // VW: dwords of a value row that a lane loads
     __shared__ float s_ml[4][16][3];
     __shared__ float s_o[4][16][HDP + 4];
-    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, n = l & 15, g = l >> 4;
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 15, g = l >> 4;
     unsigned id = blockIdx.x;
     const int split = id % a.splits;
     id /= a.splits;
@@ -152,19 +183,19 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
                 top = fmaxf(top, fabsf(x[j][e]));
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const int e2 = down_shift(top);
+        top = max_rows(top);
+        const int e2 = range_shift(top);
         to_score = ldexpf(a.scale_log2, -e2);
 #pragma unroll
-        for (int j = 0; j < KJ; ++j)
+        for (int j = 0; j < 2 * KJ; ++j) {
+            float y[8];
+            f16x8 part[PARTS];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float y = ldexpf(x[j][e], e2);
-                const _Float16 hi = (_Float16)y;
-                qf[0][2 * j + e / 8][e % 8] = hi;
-                if constexpr (PARTS == 2) qf[1][2 * j + e / 8][e % 8] = (_Float16)(y - (float)hi);
-            }
+            for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[j / 2][8 * (j % 2) + e], e2);
+            split_f16<PARTS>(y, part);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) qf[p][j] = part[p];
+        }
     }
 
     f32x4 o[NT];
@@ -172,87 +203,131 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
     for (int t = 0; t < NT; ++t) o[t] = f32x4{0, 0, 0, 0};
     float m = kNegInf, lsum = 0.0f, vref = 0.0f;
 
+    // Byte offsets of this lane's loads inside 16 tokens' rows. Channels past the head dimension are read
+    // from the row's start: queries are 0 there, and outputs are not stored.
+    const unsigned hd = (unsigned)a.hd;
+    unsigned koff[KJ], voff[4];
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) koff[j] = n * hd + (64u * j + 16u * g < hd ? 64u * j + 16u * g : 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) voff[i] = (4u * g + i) * hd + ((unsigned)(NT * n) < hd ? (unsigned)(NT * n) : 0u);
+
     const int page_mask = (1 << a.page_shift) - 1;
     const int32_t *table = a.table + (size_t)r * a.max_pages;
-    for (int t0 = begin + 32 * w; t0 < end; t0 += 128) {
-        // 2 x 16 tokens, each 16 in one page
+    // 2 x 16 tokens, each 16 in one page; the next tile's are loaded while this one's are used
+    struct Tile {
         float ks[2], vs[2];
         bool there[2];
         u32x4 kw[2][KJ];
         uint32_t vw[VW][8];
+    };
+    // (the page ids of a tile are fetched while the tile before it is loaded; past the end the last
+    // tokens are loaded again, so that every tile has the same loads in flight behind it)
+    const int t_last = max(end - 1, begin) & ~15;
+    int page0, page1;
+    auto fetch = [&](int t0) {
+        page0 = table[min(t0, t_last) >> a.page_shift];
+        page1 = table[min(t0 + 16, t_last) >> a.page_shift];
+    };
+    auto load = [&](int t0, Tile &x) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int t = t0 + 16 * s;
-            const int page = t < end ? table[t >> a.page_shift] : -1;
-            there[s] = page_ok(page, a.n_pages);
-            const size_t ph = (size_t)(there[s] ? page : 0) * a.n_kv + h;
-            ks[s] = there[s] ? a.ks[ph] : 0.0f;
-            vs[s] = there[s] ? a.vs[ph] : 0.0f;
-            const size_t row = (ph << a.page_shift) + (t & page_mask);
-            const int8_t *kp = a.k + (row + n) * a.hd, *vp = a.v + (row + 4 * g) * a.hd;
+            const int t = min(t0 + 16 * s, t_last), page = s ? page1 : page0;
+            x.there[s] = page_ok(page, a.n_pages);
+            const size_t ph = (size_t)(x.there[s] ? page : 0) * a.n_kv + h;
+            x.ks[s] = a.ks[ph];
+            x.vs[s] = a.vs[ph];
+            const size_t row = ((ph << a.page_shift) + (t & page_mask)) * hd;
+            const int8_t *kp = a.k + row, *vp = a.v + row;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                const int d = 64 * j + 16 * g;
-                kw[s][j] = d < a.hd ? *reinterpret_cast<const u32x4 *>(kp + d) : u32x4{0, 0, 0, 0};
-            }
+            for (int j = 0; j < KJ; ++j) x.kw[s][j] = *reinterpret_cast<const u32x4 *>(kp + koff[j]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = NT * n;
+                uint32_t w[VW];
+                __builtin_memcpy(w, __builtin_assume_aligned(vp + voff[i], 4 * VW), 4 * VW);
 #pragma unroll
-                for (int x = 0; x < VW; ++x)
-                    vw[x][4 * s + i] = d < a.hd ? *reinterpret_cast<const uint32_t *>(vp + (size_t)i * a.hd + d + 4 * x) : 0u;
+                for (int e = 0; e < VW; ++e) x.vw[e][4 * s + i] = w[e];
             }
         }
+    };
+    const int pos_lo = rq.len - rq.count + c0 / a.grp, pos_hi = rq.len - rq.count + (min(c0 + 16, cols) - 1) / a.grp;
+    auto use = [&](int t0, Tile &x) {
         float s[8], top = kNegInf;
+        // (tiles that every column sees whole need no comparisons)
+        const bool whole = x.there[0] && x.there[1] && t0 + 31 <= pos_lo && pos_hi - t0 < a.window;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < KJ; ++j) {
-                const f16x8 k0 = codes8(kw[u][j].x, kw[u][j].y), k1 = codes8(kw[u][j].z, kw[u][j].w);
+                const f16x8 k0 = codes8(x.kw[u][j].x, x.kw[u][j].y), k1 = codes8(x.kw[u][j].z, x.kw[u][j].w);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[p][2 * j], acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[p][2 * j + 1], acc, 0, 0, 0);
                 }
             }
-            const float f = ks[u] * to_score;
+            const float f = x.ks[u] * to_score;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = t0 + 16 * u + 4 * g + i;
-                const bool sees = there[u] && t <= pos && pos - t < a.window;
-                s[4 * u + i] = sees ? acc[i] * f : kNegInf;
-                top = fmaxf(top, s[4 * u + i]);
+            for (int i = 0; i < 4; ++i) s[4 * u + i] = acc[i] * f;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
+                if (!(x.there[i / 4] && t <= pos && pos - t < a.window)) s[i] = kNegInf;
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float m_new = fmaxf(m, top), m_use = m_new == kNegInf ? 0.0f : m_new;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i]);
+        const float m_new = fmaxf(m, max_rows(top)), m_use = m_new == kNegInf ? 0.0f : m_new;
+        const float vs[2] = {x.there[0] ? x.vs[0] : 0.0f, x.there[1] ? x.vs[1] : 0.0f};
         const float vref_new = fmaxf(vref, fmaxf(vs[0], vs[1])), per = vref_new > 0.0f ? 1.0f / vref_new : 0.0f;
-        const float fade = exp2_fast(m - m_use), fade_o = fade * (vref * per);
+        const float fade = exp2_fast(m - m_use), fade_o = vref == vref_new ? fade : fade * (vref * per);
+        const float vw[2] = {vs[0] * (per * kWeightScale), vs[1] * (per * kWeightScale)};
         lsum *= fade;
         f16x8 wf[PARTS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float p = s[i] == kNegInf ? 0.0f : exp2_fast(s[i] - m_use);
+            const float p = exp2_fast(s[i] - m_use);  // (unseen: 2^-inf = 0)
             lsum += p;
-            const float y = p * (vs[i / 4] * per);
-            const _Float16 hi = (_Float16)y;
-            wf[0][i] = hi;
-            if constexpr (PARTS == 2) wf[1][i] = (_Float16)(y - (float)hi);
+            s[i] = p * vw[i / 4];
         }
+        split_f16<PARTS>(s, wf);
         m = m_new;
         vref = vref_new;
+        if (__any(fade_o != 1.0f)) {
 #pragma unroll
-        for (int x = 0; x < VW; ++x)
+            for (int t = 0; t < NT; ++t) o[t] *= fade_o;
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) vw[x][i] ^= 0x80808080u;
+        for (int e = 0; e < VW; ++e)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.vw[e][i] ^= 0x80808080u;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const f16x8 vf = codes_across(vw[t / 4], t % 4);
-            o[t] *= fade_o;
+            const f16x8 vf = codes_across(x.vw[t / 4], t % 4);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wf[p], o[t], 0, 0, 0);
+        }
+    };
+    int t0 = begin + 32 * w;
+    if (t0 < end) {
+        Tile tiles[2];
+        fetch(t0);
+        load(t0, tiles[0]);
+        fetch(t0 + 128);
+        while (true) {
+            load(t0 + 128, tiles[1]);
+            fetch(t0 + 256);
+            use(t0, tiles[0]);
+            t0 += 128;
+            if (t0 >= end) break;
+            load(t0 + 128, tiles[0]);
+            fetch(t0 + 256);
+            use(t0, tiles[1]);
+            t0 += 128;
+            if (t0 >= end) break;
         }
     }
 
@@ -269,7 +344,7 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
     for (int i = 0; i < 4; ++i) m_all = fmaxf(m_all, s_ml[i][n][0]);
     const float m_use = m_all == kNegInf ? 0.0f : m_all;
     // (NaN scores leave m at -inf but make the sum NaN: it must not be multiplied away)
-    const float mine = m == kNegInf ? (__builtin_isnan(lsum) ? lsum : 0.0f) : exp2_fast(m - m_use) * vref * kCodeScale;
+    const float mine = m == kNegInf ? (__builtin_isnan(lsum) ? lsum : 0.0f) : exp2_fast(m - m_use) * vref * (kCodeScale / kWeightScale);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
