@@ -619,7 +619,7 @@ jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent
                            int32_t *lens_out, int32_t *table_out);
 
 /* One layer's cache. Codes of page p, kv head h, row t and channel d at ((p * n_kv + h) * page + t) * head_dim + d;
- * a value is code * scale[p * n_kv + h]. */
+ * a value is code * scale[p * n_kv + h], scales 0 or more. */
 typedef struct jk_kv_q8 {
     size_t n_pages, page; /* as in jk_paged */
     size_t n_kv;          /* kv heads */

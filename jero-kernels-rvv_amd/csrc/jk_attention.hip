@@ -1,142 +1,11 @@
-// jk_attention.hip -- attention of a step's queries over the paged 8-bit cache.
-//
-// Notation: a column is one (query token, query head) pair of a kv head's group; the columns of a request
-// and kv head are numbered token-major, c = token * group + head of the group.
-//
-// One pass over the keys with a running maximum m and sum l per column:
-//   s_j = scale q.k_j,  p_j = exp(s_j - m),  l = sum p_j,  o = sum p_j v_j / l
-// with k_j = ks * codes and v_j = vs * codes, ks and vs one number per page and head. The products run on f16
-// matrix instructions: codes are exact in f16, ks multiplies the finished score, and vs joins the
-// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j <= 1 whatever the values' size (held times 2^14); o is
-// rescaled by r like by m. Scores are computed transposed (rows = tokens), so a lane that holds a column's
-// scores of four consecutive tokens holds them just as the second product's operand wants them: the order
-// of the tokens inside a matrix instruction is free as long as both of its operands agree on it.
+// jk_attention.hip -- attention over the paged 8-bit cache: the kernel for few columns (a decode step, drafted tokens), the
+// joining of split keys, and the entry points.
 #include <algorithm>
 #include <cmath>
 
-#include "jk_device.hpp"
+#include "jk_attention.hpp"
 
 namespace jk {
-
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-constexpr float kNegInf = -__builtin_inff();
-constexpr float kCodeScale = 512.0f;  // a code becomes code / 512 in f16 (code_pair)
-// Queries and weights are held in f16 with their largest values near 2^14, so that what is 2^-28 of those is still a
-// normal number, and the low parts of f32 ones keep their bits: weights are p_j vs / r times this.
-constexpr float kWeightScale = 16384.0f;
-
-struct AttnDev {
-    const void *q;
-    void *out;
-    size_t qt, qh, ot, oh;  // strides in elements
-    bool q_vec, out_vec;
-    int n_tokens, n_heads, n_kv, grp, hd, page_shift, n_pages, max_pages, n_requests, max_new;
-    const int32_t *q_start, *lens, *table;
-    const int8_t *k, *v;
-    const float *ks, *vs;
-    float scale_log2;  // scale * log2(e) * kCodeScale
-    int window;        // INT_MAX: none
-    int tiles, splits;
-    float *part_o;   // [n_tokens * n_heads][splits][hd]: sums over a split, not yet divided by l
-    float2 *part_ml;  // [n_tokens * n_heads][splits]: m (in powers of two) and l
-};
-
-// The tokens of a request in the step, [first, last) of q, and the length of its cache, as far as the arrays go.
-struct Req {
-    int first, count, len;
-};
-__device__ __forceinline__ Req request_of(const AttnDev &a, int r) {
-    Req q;
-    q.first = min(max(a.q_start[r], 0), a.n_tokens);
-    q.count = min(max(a.q_start[r + 1], q.first), a.n_tokens) - q.first;
-    q.len = (int)min((long)max(a.lens[r], 0), (long)a.max_pages << a.page_shift);
-    return q;
-}
-
-// The keys that columns [c0, c1) of a request can see, [lo, hi) with lo a multiple of 32, cut into pieces of
-// `chunk` (a multiple of 128) over at most `splits` workgroups.
-constexpr int kMinChunk = 256;
-struct Span {
-    int lo, hi, chunk, active;
-};
-__device__ __forceinline__ Span span_of(const AttnDev &a, const Req &q, int c0, int c1) {
-    Span s;
-    const int p0 = q.len - q.count + c0 / a.grp, p1 = q.len - q.count + (c1 - 1) / a.grp;
-    s.lo = max(p0 < a.window ? 0 : p0 - a.window + 1, 0) & ~31;
-    s.hi = max(min(q.len, p1 + 1), s.lo);
-    const int n = s.hi - s.lo;
-    s.chunk = max(kMinChunk, ((n + a.splits - 1) / a.splits + 127) & ~127);
-    s.active = max(1, (n + s.chunk - 1) / s.chunk);
-    return s;
-}
-
-// Two biased codes (code + 128 in the low byte of each half) as f16 pair code / 512: a half 0x00bb is the
-// subnormal bb * 2^-24, and bb * 2^-24 * 2^15 - 128 / 512 = code / 512 exactly.
-__device__ __forceinline__ f16x2 code_pair(uint32_t halves) {
-    const f16x2 x = __builtin_bit_cast(f16x2, halves);
-    const f16x2 up = {(_Float16)32768.0f, (_Float16)32768.0f}, bias = {(_Float16)-0.25f, (_Float16)-0.25f};
-    return __builtin_elementwise_fma(x, up, bias);
-}
-__device__ __forceinline__ f16x8 codes8(uint32_t w0, uint32_t w1) {
-    union {
-        f16x2 p[4];
-        f16x8 v;
-    } u;
-    w0 ^= 0x80808080u;
-    w1 ^= 0x80808080u;
-    u.p[0] = code_pair(__builtin_amdgcn_perm(0u, w0, 0x0c010c00u));
-    u.p[1] = code_pair(__builtin_amdgcn_perm(0u, w0, 0x0c030c02u));
-    u.p[2] = code_pair(__builtin_amdgcn_perm(0u, w1, 0x0c010c00u));
-    u.p[3] = code_pair(__builtin_amdgcn_perm(0u, w1, 0x0c030c02u));
-    return u.v;
-}
-// Byte b of eight dwords (biased already): the codes of one channel of eight tokens.
-__device__ __forceinline__ f16x8 codes_across(const uint32_t *w, int b) {
-    union {
-        f16x2 p[4];
-        f16x8 v;
-    } u;
-    const uint32_t sel = 0x0c000c00u | (uint32_t)((4 + b) << 16) | (uint32_t)b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u.p[i] = code_pair(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], sel));
-    return u.v;
-}
-
-// Maximum over the four lanes of a column (lanes 16 apart).
-__device__ __forceinline__ float max_rows(float v) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// Eight f32 values as f16 (PARTS 1), or as two f16 that add up to 22 bits of them. The low part is taken from the very
-// number that the high part became: the empty asm keeps the compiler from converting y a second time with another
-// instruction, which was seen to round some values to the other neighbour.
-template <int PARTS>
-__device__ __forceinline__ void split_f16(const float *y, f16x8 *out) {
-    union {
-        f16x8 v;
-        uint32_t w[4];
-    } hi;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) hi.v[i] = (_Float16)y[i];
-    if constexpr (PARTS == 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) asm("" : "+v"(hi.w[i]));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[1][i] = (_Float16)(y[i] - (float)hi.v[i]);
-    }
-    out[0] = hi.v;
-}
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Power of two that brings a row whose largest |value| is m to [2^13, 2^14) (zeros, infinities and NaN: any).
-__device__ __forceinline__ int range_shift(float m) { return 140 - (int)((__float_as_uint(m) >> 23) & 255u); }
 
 // Up to 16 columns of one request and kv head over one split of its keys, by four waves that take 32 tokens in
 // turn; their sums are joined in LDS. A lane (n = lane % 16, g = lane / 16) holds of column n: the query's
@@ -160,43 +29,10 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
 
     const Req rq = request_of(a, r);
     const int cols = min(rq.count, a.max_new) * a.grp, c0 = ct * 16;
-    if (c0 >= cols) return;
+    if (c0 >= cols || cols > a.few_cols) return;
     const Span sp = span_of(a, rq, c0, min(c0 + 16, cols));
     if (split >= sp.active) return;
     const int begin = sp.lo + split * sp.chunk, end = min(sp.hi, begin + sp.chunk);
-
-    // this lane's column
-    const int c = min(c0 + n, cols - 1), token = rq.first + c / a.grp, head = h * a.grp + c % a.grp;
-    const int pos = rq.len - rq.count + c / a.grp;  // sees tokens (pos - window, pos]
-    f16x8 qf[PARTS][2 * KJ];
-    float to_score;
-    {
-        const typename T::raw *q = static_cast<const typename T::raw *>(a.q) + (size_t)token * a.qt + (size_t)head * a.qh;
-        float x[KJ][16], top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) {
-            const int d = 64 * j + 16 * g;
-            if (d < a.hd) load_up<T, 16>(q + d, a.q_vec, x[j]);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                if (d >= a.hd) x[j][e] = 0.0f;
-                top = fmaxf(top, fabsf(x[j][e]));
-            }
-        }
-        top = max_rows(top);
-        const int e2 = range_shift(top);
-        to_score = ldexpf(a.scale_log2, -e2);
-#pragma unroll
-        for (int j = 0; j < 2 * KJ; ++j) {
-            float y[8];
-            f16x8 part[PARTS];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[j / 2][8 * (j % 2) + e], e2);
-            split_f16<PARTS>(y, part);
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) qf[p][j] = part[p];
-        }
-    }
 
     f32x4 o[NT];
 #pragma unroll
@@ -250,6 +86,49 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
             }
         }
     };
+    // (the first tile's loads go out before the queries are looked at)
+    Tile tiles[2];
+    int t0 = begin + 32 * w;
+    if (t0 < end) {
+        fetch(t0);
+        load(t0, tiles[0]);
+        fetch(t0 + 128);
+    }
+
+    // this lane's column
+    const int c = min(c0 + n, cols - 1), token = rq.first + c / a.grp, head = h * a.grp + c % a.grp;
+    const int pos = rq.len - rq.count + c / a.grp;  // sees tokens (pos - window, pos]
+    f16x8 qf[PARTS][2 * KJ];
+    float to_score;
+    {
+        const typename T::raw *q = static_cast<const typename T::raw *>(a.q) + (size_t)token * a.qt + (size_t)head * a.qh;
+        float x[KJ][16], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+            const int d = 64 * j + 16 * g;
+            if (d < a.hd) load_up<T, 16>(q + d, a.q_vec, x[j]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (d >= a.hd) x[j][e] = 0.0f;
+                top = fmaxf(top, fabsf(x[j][e]));
+            }
+        }
+        top = max_rows(top);
+        const int e2 = range_shift(top);
+        to_score = ldexpf(a.scale_log2, -e2);
+#pragma unroll
+        for (int j = 0; j < 2 * KJ; ++j) {
+            float y[8];
+            f16x8 part[PARTS];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[j / 2][8 * (j % 2) + e], e2);
+            split_f16<PARTS>(y, part);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) qf[p][j] = part[p];
+        }
+    }
+
+
     const int pos_lo = rq.len - rq.count + c0 / a.grp, pos_hi = rq.len - rq.count + (min(c0 + 16, cols) - 1) / a.grp;
     auto use = [&](int t0, Tile &x) {
         float s[8], top = kNegInf;
@@ -311,12 +190,7 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
             for (int p = 0; p < PARTS; ++p) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wf[p], o[t], 0, 0, 0);
         }
     };
-    int t0 = begin + 32 * w;
     if (t0 < end) {
-        Tile tiles[2];
-        fetch(t0);
-        load(t0, tiles[0]);
-        fetch(t0 + 128);
         while (true) {
             load(t0 + 128, tiles[1]);
             fetch(t0 + 256);
@@ -374,18 +248,21 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
             for (int e = 0; e < 8; ++e) y[e] *= inv;
             store_down<T, 8>(static_cast<typename T::raw *>(a.out) + (size_t)tok * a.ot + (size_t)hq * a.oh + d, a.out_vec, y);
         } else {
-            const size_t at = ((size_t)tok * a.n_heads + hq) * a.splits + split;
+            const size_t at = ((size_t)tok * a.n_heads + hq) * a.pitch + split;
             store_down<F32, 8>(a.part_o + at * a.hd + d, true, y);
             if (d == 0) a.part_ml[at] = make_float2(s_ml[1][col][2], lc);
         }
     }
 }
 
-// Joins the splits of one column a wave: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
-template <typename T>
+// Joins the splits of one column a wave: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. The lanes first take a split each
+// (their factors), then four channels each, with G groups of lanes on every G-th split; four splits' loads in flight.
+template <typename T, int HDP>
 __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
-    const int l = threadIdx.x & 63;
-    const long unit = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int LP = HDP / 4, G = 64 / LP;
+    __shared__ float s_f[4][kMaxSplits];
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long unit = (long)blockIdx.x * 4 + w;
     if (unit >= (long)a.n_tokens * a.n_heads) return;
     const int token = (int)(unit / a.n_heads), head = (int)(unit % a.n_heads), h = head / a.grp;
     // the request of the token
@@ -398,29 +275,46 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
     }
     const Req rq = request_of(a, lo);
     const int i = token - rq.first;
-    const int cols = min(rq.count, a.max_new) * a.grp, c = i * a.grp + (head - h * a.grp), c0 = c & ~15;
+    const int cols = min(rq.count, a.max_new) * a.grp, c = i * a.grp + (head - h * a.grp);
     if (i < 0 || c >= cols) return;
-    const Span sp = span_of(a, rq, c0, min(c0 + 16, cols));
+    a.splits = cols <= a.few_cols ? a.few_splits : a.many_splits;
+    a.chunk = cols <= a.few_cols ? a.few_chunk : a.many_chunk;
+    const int tile = cols <= a.few_cols ? 16 : a.many_cols, c0 = c / tile * tile;
+    const Span sp = span_of(a, rq, c0, min(c0 + tile, cols));
     if (sp.active == 1) return;  // (written whole)
-    const size_t at = (size_t)unit * a.splits;
-    float m = kNegInf;
-    for (int s = 0; s < sp.active; ++s) m = fmaxf(m, a.part_ml[at + s].x);
+    const size_t at = (size_t)unit * a.pitch;
+    float m = kNegInf, lsum = 0.0f;
+    for (int s = l; s < sp.active; s += 64) m = fmaxf(m, a.part_ml[at + s].x);
+    m = wave_max64_dpp(m);
     const float m_use = m == kNegInf ? 0.0f : m;
-    float y[4] = {0, 0, 0, 0}, lsum = 0.0f;
-    for (int s = 0; s < sp.active; ++s) {
+    for (int s = l; s < sp.active; s += 64) {
         const float2 ml = a.part_ml[at + s];
         const float f = exp2_fast(ml.x - m_use);
+        s_f[w][s] = f;
         lsum += ml.x == kNegInf ? ml.y : ml.y * f;  // (0, or NaN)
-        if (4 * l < a.hd) {
-            const float4 o = *reinterpret_cast<const float4 *>(a.part_o + (at + s) * a.hd + 4 * l);
-            y[0] = fmaf(o.x, f, y[0]), y[1] = fmaf(o.y, f, y[1]), y[2] = fmaf(o.z, f, y[2]), y[3] = fmaf(o.w, f, y[3]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) lsum += __shfl_xor(lsum, o, 64);
+    wave_lds_sync();
+    const int d = 4 * (l % LP);
+    float4 y = make_float4(0, 0, 0, 0);
+    if (d < a.hd) {
+#pragma unroll 4
+        for (int s = l / LP; s < sp.active; s += G) {
+            const float4 o = *reinterpret_cast<const float4 *>(a.part_o + (at + s) * a.hd + d);
+            const float f = s_f[w][s];
+            y.x = fmaf(o.x, f, y.x), y.y = fmaf(o.y, f, y.y), y.z = fmaf(o.z, f, y.z), y.w = fmaf(o.w, f, y.w);
         }
     }
-    const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-    if (4 * l < a.hd) {
-        typename T::raw *out = static_cast<typename T::raw *>(a.out) + (size_t)token * a.ot + (size_t)head * a.oh + 4 * l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = T::down(y[e] * inv);
+    for (int o = LP; o < 64; o <<= 1) {
+        y.x += __shfl_xor(y.x, o, 64), y.y += __shfl_xor(y.y, o, 64);
+        y.z += __shfl_xor(y.z, o, 64), y.w += __shfl_xor(y.w, o, 64);
+    }
+    if (l < LP && d < a.hd) {
+        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+        typename T::raw *out = static_cast<typename T::raw *>(a.out) + (size_t)token * a.ot + (size_t)head * a.oh + d;
+        out[0] = T::down(y.x * inv), out[1] = T::down(y.y * inv), out[2] = T::down(y.z * inv), out[3] = T::down(y.w * inv);
     }
 }
 
@@ -438,33 +332,73 @@ static jk_status attn_check(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
     return JK_OK;
 }
 
-// How many workgroups share the keys of a column tile: enough to fill the GPU twice over, and no more than
-// kMaxChunk keys each, so that a long request in a batch of short ones does not hold up the launch.
-constexpr size_t kMaxChunk = 4096, kMaxSplits = 256;
-static size_t attn_tiles(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
-    return (std::min(a->max_new, a->n_tokens) * (a->n_heads / c->n_kv) + 15) / 16;
+// How a call is cut up. Requests of up to kFewCols columns go to the rows kernel, sixteen columns a workgroup; longer ones to
+// the prompt kernel. (One request, 32 query and 8 kv heads of 128, bf16, rows against prompt kernel: 128 new tokens after 2000 20 and
+// 30 us; 512 after none 19 and 20 us, after 4000 105 and 70 us; 2048 after none 115 and 64 us.) A call that can hold both
+// launches both (the counts are known on the device only), except that the prompt kernel takes a lone request
+// whatever its length turns out to be.
+// The prompt kernel takes 256 columns a workgroup (one a CU, 159 us for the 4096-token prompt against 175 with 128) where
+// there are two tiles a CU to level out their lengths, else 128 (two a CU: 64 us for 2048 tokens against 96).
+// Where there are fewer tiles than places, their keys are cut into chunks of one size for the whole call, a place's share of the work,
+// so that the last ones are not left with a long request or with a prompt's last tiles, which see the most keys. Up to kWholeLen
+// keys are not cut in the rows kernel: the second launch costs more than it saves (three requests of up to 700 keys 9 us whole, 13
+// in two; one of 1000 12.4 and 14; of 2000 17.5 and 14).
+constexpr size_t kFewCols = 1024, kFewColsF32 = 2048, kMixedCols = 64, kMinChunk = 256, kMinPromptChunk = 512, kWholeLen = 1024;
+struct AttnPlan {
+    size_t few_tiles, few_splits, few_chunk, many_cols, many_tiles, many_splits, many_chunk, few_cols, pitch;
+};
+static AttnPlan attn_plan(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
+    AttnPlan p{};
+    const size_t new_tokens = std::min(a->max_new, a->n_tokens), cols = new_tokens * (a->n_heads / c->n_kv);
+    const size_t heads = a->n_requests * c->n_kv, ncu = (size_t)cu_count();
+    size_t len = std::min(a->max_len, a->max_pages * c->page);
+    if (a->window) len = std::min(len, a->window + new_tokens);
+    auto cut = [&](size_t share, size_t least, size_t *splits, size_t *chunk) {
+        *chunk = std::max({share, least, (len + kMaxSplits - 1) / kMaxSplits});
+        *chunk = (*chunk + 127) / 128 * 128;
+        *splits = std::max<size_t>(1, (len + *chunk - 1) / *chunk);
+    };
+    const size_t few = a->dtype == JK_F32 ? kFewColsF32 : kFewCols;
+    p.few_cols = cols <= few ? few : a->n_requests == 1 ? 0 : kMixedCols;
+    p.few_splits = p.many_splits = p.few_chunk = p.many_chunk = 1;
+    if (p.few_cols) {
+        p.few_tiles = (std::min(cols, p.few_cols) + 15) / 16;
+        cut(heads * p.few_tiles * len / ncu, len <= kWholeLen ? kWholeLen : kMinChunk, &p.few_splits, &p.few_chunk);
+    }
+    if (cols > p.few_cols) {
+        p.many_cols = c->head_dim <= 128 && heads * ((cols + 255) / 256) >= 2 * ncu ? 256 : 128;
+        p.many_tiles = (cols + p.many_cols - 1) / p.many_cols;
+        const size_t tiles = heads * p.many_tiles, places = p.many_cols == 128 ? 2 * ncu : ncu;
+        if (tiles < places)
+            cut(tiles * (len - std::min(len, new_tokens) / 2) / places, kMinPromptChunk, &p.many_splits, &p.many_chunk);
+    }
+    p.pitch = std::max(p.few_splits, p.many_splits);
+    return p;
 }
-static size_t attn_splits(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
-    const size_t units = std::max<size_t>(1, a->n_requests * attn_tiles(c, a) * c->n_kv);
-    const size_t len = std::min(a->max_len, a->max_pages * c->page);
-    const size_t most = std::max<size_t>(1, std::min<size_t>(kMaxSplits, (len + kMinChunk - 1) / kMinChunk));
-    const size_t want = std::max((2 * (size_t)cu_count() + units - 1) / units, (len + kMaxChunk - 1) / kMaxChunk);
-    return std::min(most, std::max<size_t>(1, want));
-}
-static size_t attn_ws_bytes(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
-    const size_t s = attn_splits(c, a);
-    return s == 1 ? 0 : a->n_tokens * a->n_heads * s * (c->head_dim * 4 + 8);
+static size_t attn_ws_bytes(const jk_kv_q8 *c, const jk_attn_q8_args *a, const AttnPlan &p) {
+    return p.pitch == 1 ? 0 : a->n_tokens * a->n_heads * p.pitch * (c->head_dim * 4 + 8);
 }
 
 template <typename T, int PARTS>
-static jk_status launch_attn(hipStream_t s, const AttnDev &d, unsigned grid) {
-    if (d.hd <= 64) hipLaunchKernelGGL((attn_q8_rows_kernel<T, 64, PARTS>), dim3(grid), dim3(256), 0, s, d);
-    else if (d.hd <= 128) hipLaunchKernelGGL((attn_q8_rows_kernel<T, 128, PARTS>), dim3(grid), dim3(256), 0, s, d);
-    else hipLaunchKernelGGL((attn_q8_rows_kernel<T, 256, PARTS>), dim3(grid), dim3(256), 0, s, d);
-    JK_TRY(check_launch("attn_q8_rows_kernel"));
-    if (d.splits == 1) return JK_OK;
+static jk_status launch_attn(hipStream_t s, int dtype, AttnDev d, const AttnPlan &p) {
+    const size_t units = (size_t)d.n_requests * d.n_kv;
+    if (p.few_tiles) {
+        d.tile_cols = 16, d.tiles = (int)p.few_tiles, d.splits = d.few_splits, d.chunk = d.few_chunk;
+        const dim3 grid((unsigned)(units * p.few_tiles * p.few_splits));
+        if (d.hd <= 64) hipLaunchKernelGGL((attn_q8_rows_kernel<T, 64, PARTS>), grid, dim3(256), 0, s, d);
+        else if (d.hd <= 128) hipLaunchKernelGGL((attn_q8_rows_kernel<T, 128, PARTS>), grid, dim3(256), 0, s, d);
+        else hipLaunchKernelGGL((attn_q8_rows_kernel<T, 256, PARTS>), grid, dim3(256), 0, s, d);
+        JK_TRY(check_launch("attn_q8_rows_kernel"));
+    }
+    if (p.many_tiles) {
+        d.tile_cols = d.many_cols, d.tiles = (int)p.many_tiles, d.splits = d.many_splits, d.chunk = d.many_chunk;
+        JK_TRY(launch_attn_prompt(s, dtype, d));
+    }
+    if (p.pitch == 1) return JK_OK;
     const unsigned blocks = (unsigned)(((size_t)d.n_tokens * d.n_heads + 3) / 4);
-    hipLaunchKernelGGL(attn_q8_join_kernel<T>, dim3(blocks), dim3(256), 0, s, d);
+    if (d.hd <= 64) hipLaunchKernelGGL((attn_q8_join_kernel<T, 64>), dim3(blocks), dim3(256), 0, s, d);
+    else if (d.hd <= 128) hipLaunchKernelGGL((attn_q8_join_kernel<T, 128>), dim3(blocks), dim3(256), 0, s, d);
+    else hipLaunchKernelGGL((attn_q8_join_kernel<T, 256>), dim3(blocks), dim3(256), 0, s, d);
     return check_launch("attn_q8_join_kernel");
 }
 
@@ -475,7 +409,7 @@ using namespace jk;
 extern "C" {
 
 size_t jk_attn_q8_workspace_bytes(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
-    return attn_check(c, a) == JK_OK ? attn_ws_bytes(c, a) : 0;
+    return attn_check(c, a) == JK_OK ? attn_ws_bytes(c, a, attn_plan(c, a)) : 0;
 }
 
 jk_status jk_attn_q8(jk_stream s, const jk_kv_q8 *c, const jk_attn_q8_args *a, void *ws, size_t ws_bytes) {
@@ -504,20 +438,23 @@ jk_status jk_attn_q8(jk_stream s, const jk_kv_q8 *c, const jk_attn_q8_args *a, v
     d.k = c->k, d.v = c->v, d.ks = c->k_scale, d.vs = c->v_scale;
     d.scale_log2 = a->scale * 1.44269504088896340736f * kCodeScale;
     d.window = a->window == 0 || a->window > (size_t)INT32_MAX ? INT32_MAX : (int)a->window;
-    d.tiles = (int)attn_tiles(c, a), d.splits = (int)attn_splits(c, a);
-    const size_t need = attn_ws_bytes(c, a);
+    const AttnPlan plan = attn_plan(c, a);
+    d.few_cols = (int)plan.few_cols, d.few_splits = (int)plan.few_splits, d.few_chunk = (int)plan.few_chunk;
+    d.many_cols = (int)plan.many_cols, d.many_splits = (int)plan.many_splits, d.many_chunk = (int)plan.many_chunk;
+    d.pitch = (int)plan.pitch;
+    const size_t need = attn_ws_bytes(c, a, plan);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
         return fail(JK_TENSOR_BOUNDS, "attn_q8: workspace of %zu bytes at %p: %zu needed, 16-byte aligned", ws_bytes, ws,
                     need);
     d.part_o = static_cast<float *>(ws);
-    d.part_ml = reinterpret_cast<float2 *>(d.part_o + (need ? a->n_tokens * a->n_heads * d.splits * c->head_dim : 0));
-    const size_t grid = a->n_requests * d.tiles * c->n_kv * d.splits;
-    if (grid >= (size_t)1 << 24)
+    d.part_ml = reinterpret_cast<float2 *>(d.part_o + (need ? a->n_tokens * a->n_heads * plan.pitch * c->head_dim : 0));
+    const size_t units = a->n_requests * c->n_kv, most = (size_t)1 << 24;
+    if (units * plan.few_tiles * plan.few_splits >= most || units * plan.many_tiles * plan.many_splits >= most)
         return fail(JK_TENSOR_BOUNDS, "attn_q8: %zu requests of up to %zu new tokens and %zu kv heads are too many for one call",
                     a->n_requests, a->max_new, c->n_kv);
-    if (a->dtype == JK_F32) return launch_attn<F32, 2>((hipStream_t)s, d, (unsigned)grid);
-    if (a->dtype == JK_F16) return launch_attn<F16, 1>((hipStream_t)s, d, (unsigned)grid);
-    return launch_attn<BF16, 1>((hipStream_t)s, d, (unsigned)grid);
+    if (a->dtype == JK_F32) return launch_attn<F32, 2>((hipStream_t)s, a->dtype, d, plan);
+    if (a->dtype == JK_F16) return launch_attn<F16, 1>((hipStream_t)s, a->dtype, d, plan);
+    return launch_attn<BF16, 1>((hipStream_t)s, a->dtype, d, plan);
 }
 
 }  // extern "C"

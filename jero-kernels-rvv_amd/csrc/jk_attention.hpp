@@ -1,0 +1,168 @@
+// jk_attention.hpp -- attention of a step's queries over the paged 8-bit cache: what its two kernels (jk_attention.hip,
+// jk_attention_prompt.hip) share.
+//
+// Notation: a column is one (query token, query head) pair of a kv head's group; the columns of a request
+// and kv head are numbered token-major, c = token * group + head of the group.
+//
+// One pass over the keys with a running maximum m and sum l per column:
+//   s_j = scale q.k_j,  p_j = exp(s_j - m),  l = sum p_j,  o = sum p_j v_j / l
+// with k_j = ks * codes and v_j = vs * codes, ks and vs one number per page and head. The products run on f16
+// matrix instructions: codes are exact in f16, ks multiplies the finished score, and vs joins the
+// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j <= 1 whatever the values' size (held times 2^14); o is
+// rescaled by r like by m. Scores are computed transposed (rows = tokens), so a lane that holds a column's
+// scores of four consecutive tokens holds them just as the second product's operand wants them: the order
+// of the tokens inside a matrix instruction is free as long as both of its operands agree on it.
+#pragma once
+
+#include "jk_device.hpp"
+
+namespace jk {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kCodeScale = 512.0f;  // a code becomes code / 512 in f16 (code_pair)
+// Queries and weights are held in f16 with their largest values near 2^14, so that what is 2^-28 of those is still a
+// normal number, and the low parts of f32 ones keep their bits: weights are p_j vs / r times this.
+constexpr float kWeightScale = 16384.0f;
+
+struct AttnDev {
+    const void *q;
+    void *out;
+    size_t qt, qh, ot, oh;  // strides in elements
+    bool q_vec, out_vec;
+    int n_tokens, n_heads, n_kv, grp, hd, page_shift, n_pages, max_pages, n_requests, max_new;
+    const int32_t *q_start, *lens, *table;
+    const int8_t *k, *v;
+    const float *ks, *vs;
+    float scale_log2;  // scale * log2(e) * kCodeScale
+    int window;        // INT_MAX: none
+    int tile_cols, tiles;  // columns a workgroup takes, column tiles of a request
+    int splits, chunk;     // workgroups that share a tile's keys, and how many keys each takes
+    // requests of at most few_cols columns are the rows kernel's, the others the prompt kernel's (each launch sees all requests);
+    // the joining launch needs both kernels' tiles and splits
+    int few_cols, few_splits, few_chunk, many_cols, many_splits, many_chunk;
+    int pitch;       // splits that the parts of a row have room for
+    float *part_o;   // [n_tokens * n_heads][pitch][hd]: sums over a split, not yet divided by l
+    float2 *part_ml;  // [n_tokens * n_heads][pitch]: m (in powers of two) and l
+};
+
+// The tokens of a request in the step, [first, last) of q, and the length of its cache, as far as the arrays go.
+struct Req {
+    int first, count, len;
+};
+__device__ __forceinline__ Req request_of(const AttnDev &a, int r) {
+    Req q;
+    q.first = min(max(a.q_start[r], 0), a.n_tokens);
+    q.count = min(max(a.q_start[r + 1], q.first), a.n_tokens) - q.first;
+    q.len = (int)min((long)max(a.lens[r], 0), (long)a.max_pages << a.page_shift);
+    return q;
+}
+
+// The keys that columns [c0, c1) of a request can see, [lo, hi) with lo a multiple of 64, cut into pieces of
+// `chunk` (a multiple of 128): the plan's, or longer ones where more than `splits` pieces would be needed.
+constexpr int kMaxSplits = 256;
+struct Span {
+    int lo, hi, chunk, active;
+};
+__device__ __forceinline__ Span span_of(const AttnDev &a, const Req &q, int c0, int c1) {
+    Span s;
+    const int p0 = q.len - q.count + c0 / a.grp, p1 = q.len - q.count + (c1 - 1) / a.grp;
+    s.lo = max(p0 < a.window ? 0 : p0 - a.window + 1, 0) & ~63;
+    s.hi = max(min(q.len, p1 + 1), s.lo);
+    const int n = s.hi - s.lo;
+    s.chunk = max(a.chunk, ((n + a.splits - 1) / a.splits + 127) & ~127);
+    s.active = max(1, (n + s.chunk - 1) / s.chunk);
+    return s;
+}
+
+// Two biased codes (code + 128 in the low byte of each half) as f16 pair code / 512: a half 0x00bb is the
+// subnormal bb * 2^-24, and bb * 2^-24 * 2^15 - 128 / 512 = code / 512 exactly.
+__device__ __forceinline__ f16x2 code_pair(uint32_t halves) {
+    const f16x2 x = __builtin_bit_cast(f16x2, halves);
+    const f16x2 up = {(_Float16)32768.0f, (_Float16)32768.0f}, bias = {(_Float16)-0.25f, (_Float16)-0.25f};
+    return __builtin_elementwise_fma(x, up, bias);
+}
+__device__ __forceinline__ f16x8 codes8(uint32_t w0, uint32_t w1) {
+    union {
+        f16x2 p[4];
+        f16x8 v;
+    } u;
+    w0 ^= 0x80808080u;
+    w1 ^= 0x80808080u;
+    u.p[0] = code_pair(__builtin_amdgcn_perm(0u, w0, 0x0c010c00u));
+    u.p[1] = code_pair(__builtin_amdgcn_perm(0u, w0, 0x0c030c02u));
+    u.p[2] = code_pair(__builtin_amdgcn_perm(0u, w1, 0x0c010c00u));
+    u.p[3] = code_pair(__builtin_amdgcn_perm(0u, w1, 0x0c030c02u));
+    return u.v;
+}
+// Byte b of eight dwords (biased already): the codes of one channel of eight tokens.
+__device__ __forceinline__ f16x8 codes_across(const uint32_t *w, int b) {
+    union {
+        f16x2 p[4];
+        f16x8 v;
+    } u;
+    const uint32_t sel = 0x0c000c00u | (uint32_t)((4 + b) << 16) | (uint32_t)b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u.p[i] = code_pair(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], sel));
+    return u.v;
+}
+
+// Maximum over the four lanes of a column (lanes 16 apart).
+__device__ __forceinline__ float max_rows(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Eight f32 values as f16 (PARTS 1), or as two f16 that add up to 22 bits of them. The low part is taken from the very
+// number that the high part became: the empty asm keeps the compiler from converting y a second time with another
+// instruction, which was seen to round some values to the other neighbour.
+template <int PARTS>
+__device__ __forceinline__ void split_f16(const float *y, f16x8 *out) {
+    union {
+        f16x8 v;
+        uint32_t w[4];
+    } hi;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) hi.v[i] = (_Float16)y[i];
+    if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("" : "+v"(hi.w[i]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[1][i] = (_Float16)(y[i] - (float)hi.v[i]);
+    }
+    out[0] = hi.v;
+}
+
+// Maximum and sum over the two lanes of a column (lanes 32 apart).
+__device__ __forceinline__ float max_halves(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// Byte offsets of the 16-byte pieces in a row of the LDS tiles, swizzled so that the lanes that read (or write) one piece
+// each of neighbouring rows meet different banks: keys by the token, values by the channel and the channel / 8 (their
+// writers hold every fourth channel).
+template <int HDP>
+__device__ __forceinline__ int swz_k(int piece, int token) {
+    return (piece ^ (token & (HDP / 8 - 1))) * 16;
+}
+__device__ __forceinline__ int swz_v(int piece, int channel) { return (piece ^ ((channel ^ (channel >> 3)) & 7)) * 16; }
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Power of two that brings a row whose largest |value| is m to [2^13, 2^14) (zeros, infinities and NaN: any).
+__device__ __forceinline__ int range_shift(float m) { return 140 - (int)((__float_as_uint(m) >> 23) & 255u); }
+
+// The launch of the prompt kernel for the plan that d holds (dtype: jk_dtype; tile_cols 128, or 256 for up to 128 channels).
+jk_status launch_attn_prompt(hipStream_t s, int dtype, const AttnDev &d);
+
+}  // namespace jk

@@ -239,10 +239,7 @@ struct F16 {
 struct BF16 {
     typedef uint16_t raw;
     static __device__ __forceinline__ float up(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-    static __device__ __forceinline__ uint16_t down(float v) {
-        const uint32_t b = __float_as_uint(v);
-        return __builtin_isnan(v) ? (uint16_t)((b >> 16) | 0x40u) : (uint16_t)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
-    }
+    static __device__ __forceinline__ uint16_t down(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 };
 
 // N consecutive elements (N a multiple of 8) as f32; vec: p is 16-byte aligned.

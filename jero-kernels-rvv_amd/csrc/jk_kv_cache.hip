@@ -193,6 +193,8 @@ jk_status kv_check(const char *what, const jk_kv_q8 *c) {
     if (c->n_pages == 0 || c->n_pages > (size_t)INT32_MAX / c->page)
         return fail(JK_TENSOR_BOUNDS, "%s: %zu pages of %zu tokens exceed the int32 range of slots", what, c->n_pages,
                     c->page);
+    if (c->n_pages * c->n_kv > (size_t)INT32_MAX)
+        return fail(JK_TENSOR_BOUNDS, "%s: %zu pages of %zu kv heads exceed the int32 range", what, c->n_pages, c->n_kv);
     return JK_OK;
 }
 
