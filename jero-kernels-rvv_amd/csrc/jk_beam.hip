@@ -24,6 +24,23 @@ __device__ __forceinline__ float key_value(key_t64 k) {
 }
 __device__ __forceinline__ int key_token(key_t64 k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
 
+// Largest key of the wave (all lanes active) by lane permutations: of the high words, then of the low words beside it. (The
+// shuffles of wave_max_key go through LDS: three times the latency, and a round of the joins is little else.)
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = max(v, (uint32_t)dpp_i<kDppXor1>((int)v));
+    v = max(v, (uint32_t)dpp_i<kDppXor2>((int)v));
+    v = max(v, (uint32_t)dpp_i<kDppHalfMirror>((int)v));
+    v = max(v, (uint32_t)dpp_i<kDppMirror>((int)v));
+    const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
+    const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32), e = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+    return max(max(a, b), max(c, e));
+}
+__device__ __forceinline__ key_t64 max_key(key_t64 k) {
+    const uint32_t hi = wave_max_u32((uint32_t)(k >> 32));
+    const uint32_t lo = wave_max_u32((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return ((key_t64)hi << 32) | lo;
+}
+
 struct BeamDev {
     const void *logits;
     const float *scores;
@@ -69,7 +86,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamDev a) {
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-        if (__builtin_isnan(v[i])) v[i] = -__builtin_inff();
+        v[i] = fmaxf(v[i], -__builtin_inff());  // (a NaN counts as -inf)
         top = fmaxf(top, v[i]);
     }
     const float m = wave_max64_dpp(top);
@@ -81,22 +98,48 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamDev a) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
 
-    // the width largest, one a round: each lane offers its best remaining key below the last one taken
+    // The width largest. At least `width` logits are no smaller than the width-th largest of the lanes' maxima, and for
+    // logits that are not almost all equal hardly more: those are collected and ranked by counting, each
+    // lane one of them. Where there are more than lanes, the largest are taken one a round instead.
     const size_t at = (size_t)row * a.segs + seg;
-    key_t64 last = ~0ull;
-    for (int b = 0; b < a.width; ++b) {
-        key_t64 best = 0;
+    float bar = m, rest = top;
+    for (int have = 0;;) {
+        have += __popcll(__ballot(rest == bar));
+        if (have >= a.width || bar == -__builtin_inff()) break;
+        rest = rest == bar ? -__builtin_inff() : rest;
+        bar = wave_max64_dpp(rest);
+    }
+    __shared__ key_t64 s_keys[4][64];
+    key_t64 *keys = s_keys[threadIdx.x >> 6];
+    int n_keys = 0;
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-            const key_t64 k = tok(i) < n ? argmax_key(v[i], (uint32_t)(base + tok(i))) : 0ull;
-            best = k < last && k > best ? k : best;
+    for (int i = 0; i < kPerLane; ++i) {
+        const bool in = v[i] >= bar && tok(i) < n;
+        const unsigned long long mask = __ballot(in);
+        if (mask) {
+            const int to = n_keys + __popcll(mask & ((1ull << l) - 1));
+            if (in && to < 64) keys[to] = argmax_key(v[i], (uint32_t)(base + tok(i)));
+            n_keys += __popcll(mask);
         }
-        best = wave_max_key(best);
-        if (l == 0) a.keys[at * a.width + b] = best;
-        last = best;
-        if (best == 0) {
-            for (int r = b + 1 + l; r < a.width; r += 64) a.keys[at * a.width + r] = 0;
-            break;
+    }
+    if (n_keys <= 64) {
+        wave_lds_sync();
+        const key_t64 mine = l < n_keys ? keys[l] : 0ull;
+        int rank = 0;
+        for (int i = 0; i < n_keys; ++i) rank += keys[i] > mine;
+        if (l < n_keys && rank < a.width) a.keys[at * a.width + rank] = mine;
+        if (l >= n_keys && l < a.width) a.keys[at * a.width + l] = 0;
+    } else {
+        key_t64 last = ~0ull;
+        for (int b = 0; b < a.width; ++b) {
+            key_t64 best = 0;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+                const key_t64 k = tok(i) < n ? argmax_key(v[i], (uint32_t)(base + tok(i))) : 0ull;
+                best = k < last && k > best ? k : best;
+            }
+            last = max_key(best);
+            if (l == 0) a.keys[at * a.width + b] = last;
         }
     }
     if (l == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = sum;
@@ -105,10 +148,14 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamDev a) {
 // One workgroup a group. A wave joins a row's segments: each lane holds the best untaken key of its segments
 // (their lists are in order, so that is one position each), and the row's next best is the wave's maximum. Then the
 // first wave joins the group's rows in the same way, by their totals.
-constexpr int kJoinWaves = 8;
+// The keys are staged in LDS where a row has at most kJoinKeys of them (a vocabulary of 256k at a width of 8): a round's next key
+// then comes at LDS latency.
+constexpr int kJoinWaves = 8, kJoinKeys = 1024;
+template <int NS>  // segments a lane holds (64 * NS at most)
 __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {
     __shared__ float s_total[kMaxWidth][kMaxWidth];
     __shared__ int s_tok[kMaxWidth][kMaxWidth];
+    __shared__ key_t64 s_keys[kJoinWaves][kJoinKeys];
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6, g = blockIdx.x;
     for (int b = w; b < a.width; b += kJoinWaves) {
         const size_t row = (size_t)g * a.width + b;
@@ -129,18 +176,23 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         const float lse = logf(sum), score = a.scores[row];
         const key_t64 *keys = a.keys + row * a.segs * a.width;
-        key_t64 head[kMaxSegsPerLane];
-        int taken[kMaxSegsPerLane];
+        if (a.segs * a.width <= kJoinKeys) {
+            for (int i = l; i < a.segs * a.width; i += 64) s_keys[w][i] = keys[i];
+            wave_lds_sync();
+            keys = s_keys[w];
+        }
+        key_t64 head[NS];
+        int taken[NS];
 #pragma unroll
-        for (int i = 0; i < kMaxSegsPerLane; ++i) {
+        for (int i = 0; i < NS; ++i) {
             taken[i] = 0;
             head[i] = l + 64 * i < a.segs ? keys[(size_t)(l + 64 * i) * a.width] : 0ull;
         }
         for (int r = 0; r < a.width; ++r) {
             key_t64 best = 0;
 #pragma unroll
-            for (int i = 0; i < kMaxSegsPerLane; ++i) best = head[i] > best ? head[i] : best;
-            best = wave_max_key(best);
+            for (int i = 0; i < NS; ++i) best = head[i] > best ? head[i] : best;
+            best = max_key(best);
             if (best == 0) break;
             if (l == 0) {
                 const float t = score + ((key_value(best) - m) - lse);
@@ -148,7 +200,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {
                 s_tok[b][r] = key_token(best);
             }
 #pragma unroll
-            for (int i = 0; i < kMaxSegsPerLane; ++i)
+            for (int i = 0; i < NS; ++i)
                 if (head[i] == best) {
                     ++taken[i];
                     head[i] = taken[i] < a.width ? keys[(size_t)(l + 64 * i) * a.width + taken[i]] : 0ull;
@@ -157,22 +209,29 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {
     }
     __syncthreads();
     if (w) return;
-    // lane b offers row b's next candidate; keys order by total, then by the lower row (no NaN among totals)
-    int next = 0;
+    // lane b offers row b's next candidate (keys order by total, then by the lower row; no NaN among totals), and lane r keeps what
+    // comes out r-th
+    const size_t row0 = (size_t)g * a.width;
+    const bool mine_done = l < a.width && a.done && a.done[row0 + l];
+    auto offer = [&](int at) {
+        const bool has = l < a.width && at < a.width && s_tok[l][at] >= 0;
+        return has ? argmax_key(s_total[l][at], (uint32_t)l) : 0ull;
+    };
+    int next = 0, parent = 0, pos = 0;
+    key_t64 key = offer(0);
     for (int r = 0; r < a.width; ++r) {
-        const bool has = l < a.width && next < a.width && s_tok[l][next] >= 0;
-        const key_t64 best = wave_max_key(has ? argmax_key(s_total[l][next], (uint32_t)l) : 0ull);
-        const int b = key_token(best);  // (each row has a candidate and the first of a row comes first: best != 0)
-        const int pos = __shfl(next, b, 64);
-        const size_t out = (size_t)g * a.width + r;
-        if (l == 0) {
-            const int tok = s_tok[b][pos];
-            a.scores_out[out] = s_total[b][pos];
-            a.parents[out] = b;
-            a.tokens[out] = tok;
-            if (a.done_out) a.done_out[out] = (a.done && a.done[(size_t)g * a.width + b]) || tok == a.eos;
-        }
-        if (l == b) ++next;
+        const int b = key_token(max_key(key));  // (each row has a candidate and the first of a row comes first: there is one)
+        const int at = __builtin_amdgcn_readlane(next, b);
+        if (l == r) parent = b, pos = at;
+        if (l == b) key = offer(++next);
+    }
+    const int ended = __shfl((int)mine_done, parent, 64);
+    if (l < a.width) {
+        const int tok = s_tok[parent][pos];
+        a.scores_out[row0 + l] = s_total[parent][pos];
+        a.parents[row0 + l] = parent;
+        a.tokens[row0 + l] = tok;
+        if (a.done_out) a.done_out[row0 + l] = ended || tok == a.eos;
     }
 }
 
@@ -236,7 +295,9 @@ jk_status jk_beam_select(jk_stream s, const jk_beam_args *a, void *ws, size_t ws
     else if (a->dtype == JK_F16) hipLaunchKernelGGL(beam_rows_kernel<F16>, grid, dim3(256), 0, (hipStream_t)s, d);
     else hipLaunchKernelGGL(beam_rows_kernel<BF16>, grid, dim3(256), 0, (hipStream_t)s, d);
     JK_TRY(check_launch("beam_rows_kernel"));
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a->groups), dim3(64 * kJoinWaves), 0, (hipStream_t)s, d);
+    const dim3 joins((unsigned)a->groups);
+    if (w.segs <= 64) hipLaunchKernelGGL(beam_join_kernel<1>, joins, dim3(64 * kJoinWaves), 0, (hipStream_t)s, d);
+    else hipLaunchKernelGGL(beam_join_kernel<kMaxSegsPerLane>, joins, dim3(64 * kJoinWaves), 0, (hipStream_t)s, d);
     return check_launch("beam_join_kernel");
 }
 

@@ -21,6 +21,7 @@ struct AppendArgs {
     size_t st, sh;  // strides of x in elements
     const int32_t *slots;
     int n_tokens, n_slots, n_kv, hd, page_shift;
+    int chunk;  // tokens whose runs a workgroup takes, at most 64
     bool vec;
 };
 
@@ -43,24 +44,24 @@ __device__ __forceinline__ int run_length(const AppendArgs &a, int t0) {
     }
 }
 
-// Quantizes the runs of tokens of one page that begin among tokens [CHUNK * x, CHUNK * (x + 1)) for one head
+// Quantizes the runs of tokens of one page that begin among tokens [chunk * x, chunk * (x + 1)) for one head
 // of keys or values (blockIdx.y). One pass over the new values where the run's 8-element pieces fit kHeld a thread,
 // else a second one from the caches.
-// A decode step has one-token runs in as many pages as requests, a prompt runs of whole pages. THREADS = 64, CHUNK = 1: one
-// wave a token, so a step of few tokens is spread over many CUs. THREADS = 256, CHUNK = 16: whole pages a workgroup.
+// A decode step has one-token runs in as many pages as requests, a prompt runs of whole pages: a step takes chunks of one token
+// and 64 threads, so that its few tokens are spread over many CUs, a prompt chunks of a page and 256 threads.
 constexpr int kHeld = 4;
-template <typename T, int THREADS, int CHUNK>
+template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs a) {
     typedef typename T::raw raw;
     __shared__ float s_max[THREADS / 64];
     const int tid = threadIdx.x, l = tid & 63, which = blockIdx.y / a.n_kv, h = blockIdx.y % a.n_kv;
-    const int t_first = blockIdx.x * CHUNK;
+    const int t_first = blockIdx.x * a.chunk;
     const raw *x = static_cast<const raw *>(a.x[which]);
 
     // which of the chunk's tokens begin a run
     bool begins = false;
     const int t = t_first + l;
-    if (l < CHUNK && t < a.n_tokens) {
+    if (l < a.chunk && t < a.n_tokens) {
         const int s = a.slots[t], before = t ? a.slots[t - 1] : -1;
         begins = (unsigned)s < (unsigned)a.n_slots &&
                  !(before >= 0 && (before >> a.page_shift) == (s >> a.page_shift) && s > before);
@@ -147,37 +148,62 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs a) {
     }
 }
 
-// 16 channels of one head of one slot a thread.
+// A thread turns the codes of 16 bytes of output (4 or 8) of one head and slot into values, four of them 256 apart with their
+// loads in flight together; blockIdx.y: keys, values.
+constexpr int kReadPieces = 4;
+struct ReadArgs {
+    const int8_t *codes[2];
+    const float *scale[2];
+    void *out[2];
+    const int32_t *slots;
+    unsigned pieces;  // of 16 bytes of output
+    int n_slots, n_kv, hd, page_shift;
+    bool vec;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void kv_read_kernel(const int8_t *__restrict__ k, const float *__restrict__ ks,
-                                                      const int8_t *__restrict__ v, const float *__restrict__ vs,
-                                                      const int32_t *__restrict__ slots, size_t pieces, int n_slots,
-                                                      int n_kv, int hd, int page_shift, bool vec,
-                                                      typename T::raw *k_out, typename T::raw *v_out) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= pieces) return;
-    const int per = hd / 16;
-    const size_t head_of = i / per;
-    const int c = (int)(i - head_of * per) * 16, h = (int)(head_of % n_kv);
-    const int s = slots[head_of / n_kv];
-    const bool ok = (unsigned)s < (unsigned)n_slots;
-    const size_t head = ok ? (size_t)(s >> page_shift) * n_kv + h : 0;
-    const size_t at = ((head << page_shift) + (ok ? s & ((1 << page_shift) - 1) : 0)) * hd + c;
-    auto out = [&](const int8_t *codes, const float *scale, typename T::raw *to) {
-        float y[16];
-        if (ok) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(codes + at);
-            const float d = scale[head];
+__global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
+    typedef typename T::raw raw;
+    constexpr int N = 16 / (int)sizeof(raw);
+    const int8_t *codes = a.codes[blockIdx.y];
+    const float *scale = a.scale[blockIdx.y];
+    raw *out = static_cast<raw *>(a.out[blockIdx.y]);
+    if (!out) return;
+    const unsigned first = blockIdx.x * (256 * kReadPieces) + threadIdx.x, per = a.hd / N;
+    uint32_t w[kReadPieces][N / 4];
+    float d[kReadPieces];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * d;
+    for (int k = 0; k < kReadPieces; ++k) {
+        const unsigned i = min(first + 256 * k, a.pieces - 1), head_of = i / per, c = (i - head_of * per) * N;
+        const unsigned at = head_of / a.n_kv, h = head_of - at * a.n_kv;
+        const int s = a.slots[at];
+        const bool ok = (unsigned)s < (unsigned)a.n_slots;
+        const size_t head = ok ? (size_t)(s >> a.page_shift) * a.n_kv + h : 0;
+        const size_t place = ((head << a.page_shift) + (ok ? s & ((1 << a.page_shift) - 1) : 0)) * a.hd + c;
+        __builtin_memcpy(w[k], __builtin_assume_aligned(codes + place, N), N);
+        d[k] = scale[head];
+        if (!ok) {  // (whatever its scale: 0 even beside an infinite one)
+            d[k] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N / 4; ++e) w[k][e] = 0;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kReadPieces; ++k) {
+        const unsigned i = first + 256 * k;
+        if (i >= a.pieces) return;
+        raw y[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = T::down((float)(int8_t)(w[k][e / 4] >> (8 * (e % 4))) * d[k]);
+        raw *to = out + (size_t)i * N;
+        if (a.vec) {
+            u32x4 v;
+            __builtin_memcpy(&v, y, 16);
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(to));  // (the caller's to read, not this launch's)
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = 0.0f;
+            for (int e = 0; e < N; ++e) to[e] = y[e];
         }
-        store_down<T, 16>(to + i * 16, vec, y);
-    };
-    if (k_out) out(k, ks, k_out);
-    if (v_out) out(v, vs, v_out);
+    }
 }
 
 jk_status kv_check(const char *what, const jk_kv_q8 *c) {
@@ -199,13 +225,12 @@ jk_status kv_check(const char *what, const jk_kv_q8 *c) {
 }
 
 template <typename T>
-static void launch_append(hipStream_t s, const AppendArgs &a) {
-    const unsigned heads = 2 * (unsigned)a.n_kv;
-    if (a.n_tokens <= 1024)
-        hipLaunchKernelGGL((kv_append_kernel<T, 64, 1>), dim3((unsigned)a.n_tokens, heads), dim3(64), 0, s, a);
-    else
-        hipLaunchKernelGGL((kv_append_kernel<T, 256, 16>), dim3((unsigned)((a.n_tokens + 15) / 16), heads), dim3(256), 0,
-                           s, a);
+static void launch_append(hipStream_t s, AppendArgs a) {
+    const bool step = a.n_tokens <= 1024;
+    a.chunk = step ? 1 : std::min(64, 1 << a.page_shift);
+    const dim3 grid((unsigned)((a.n_tokens + a.chunk - 1) / a.chunk), 2 * (unsigned)a.n_kv);
+    if (step) hipLaunchKernelGGL((kv_append_kernel<T, 64>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((kv_append_kernel<T, 256>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace jk
@@ -230,7 +255,7 @@ jk_status jk_kv_append_q8(jk_stream s, const jk_kv_q8 *c, const void *k, const v
     int shift = 4;
     while (((size_t)1 << shift) < c->page) ++shift;
     const AppendArgs a{{c->k, c->v}, {c->k_scale, c->v_scale}, {k, v}, st, sh, slots, (int)n_tokens,
-                       (int)(c->n_pages * c->page), (int)c->n_kv, (int)c->head_dim, shift, vec};
+                       (int)(c->n_pages * c->page), (int)c->n_kv, (int)c->head_dim, shift, 1, vec};
     if (dtype == JK_F32) launch_append<F32>((hipStream_t)s, a);
     else if (dtype == JK_F16) launch_append<F16>((hipStream_t)s, a);
     else launch_append<BF16>((hipStream_t)s, a);
@@ -246,21 +271,17 @@ jk_status jk_kv_read_q8(jk_stream s, const jk_kv_q8 *c, const int32_t *slots, si
     const size_t es = dtype_bytes(dtype);
     if ((uintptr_t)k_out % es || (uintptr_t)v_out % es)
         return fail(JK_TENSOR_BOUNDS, "kv_read_q8: outputs must be aligned to their elements");
-    if (n > (size_t)INT32_MAX / (c->n_kv * c->head_dim / 16))
-        return fail(JK_TENSOR_BOUNDS, "kv_read_q8: %zu slots are too many for one call", n);
-    const size_t pieces = n * c->n_kv * (c->head_dim / 16);
-    const bool vec = !((uintptr_t)k_out % 16) && !((uintptr_t)v_out % 16);
+    const size_t per = c->n_kv * c->head_dim * es / 16;
+    if (n > (size_t)INT32_MAX / per) return fail(JK_TENSOR_BOUNDS, "kv_read_q8: %zu slots are too many for one call", n);
     int shift = 4;
     while (((size_t)1 << shift) < c->page) ++shift;
-    const dim3 grid((unsigned)((pieces + 255) / 256));
-#define JK_READ(T)                                                                                                     \
-    hipLaunchKernelGGL(kv_read_kernel<T>, grid, dim3(256), 0, (hipStream_t)s, c->k, c->k_scale, c->v, c->v_scale, slots, \
-                       pieces, (int)(c->n_pages * c->page), (int)c->n_kv, (int)c->head_dim, shift, vec,                  \
-                       static_cast<T::raw *>(k_out), static_cast<T::raw *>(v_out))
-    if (dtype == JK_F32) JK_READ(F32);
-    else if (dtype == JK_F16) JK_READ(F16);
-    else JK_READ(BF16);
-#undef JK_READ
+    const ReadArgs a{{c->k, c->v}, {c->k_scale, c->v_scale}, {k_out, v_out}, slots, (unsigned)(n * per),
+                     (int)(c->n_pages * c->page), (int)c->n_kv, (int)c->head_dim, shift,
+                     !((uintptr_t)k_out % 16) && !((uintptr_t)v_out % 16)};
+    const dim3 grid((unsigned)((n * per + 256 * kReadPieces - 1) / (256 * kReadPieces)), 2);
+    if (dtype == JK_F32) hipLaunchKernelGGL(kv_read_kernel<F32>, grid, dim3(256), 0, (hipStream_t)s, a);
+    else if (dtype == JK_F16) hipLaunchKernelGGL(kv_read_kernel<F16>, grid, dim3(256), 0, (hipStream_t)s, a);
+    else hipLaunchKernelGGL(kv_read_kernel<BF16>, grid, dim3(256), 0, (hipStream_t)s, a);
     return check_launch("kv_read_kernel");
 }
 

@@ -43,16 +43,24 @@ __device__ __forceinline__ unsigned long long wg_scan(unsigned long long v, unsi
     return base + inc - v;
 }
 
-__device__ __forceinline__ long wg_sum(long v, long *s) {
+// Sums over the workgroup of N values per thread, with one pair of barriers. s: 17 * N words of LDS.
+template <int N>
+__device__ __forceinline__ void wg_sums(long (&v)[N], long *s) {
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
     __syncthreads();
-    if (l == 0) s[w] = v;
+    if (l == 0)
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[w * N + k] = v[k];
     __syncthreads();
-    long sum = 0;
-    for (int i = 0; i < (int)blockDim.x / 64; ++i) sum += s[i];
-    return sum;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        v[k] = 0;
+        for (int i = 0; i < (int)blockDim.x / 64; ++i) v[k] += s[i * N + k];
+    }
 }
 
 // Largest r with start[r] <= t among start[0..n) (start[0] <= t).
@@ -78,21 +86,21 @@ __device__ __forceinline__ void write_token(const StepDev &st, int t, int slot, 
     st.requests[t] = r;
 }
 
-// The plan of a step. FILL: this launch also numbers the tokens (few of them: one launch for a decode step).
-template <bool FILL>
-__global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p, const int32_t *__restrict__ n_new,
+// The plan of a step by TH threads. FILL: this launch also numbers the tokens (few of them: one launch for a decode step).
+template <bool FILL, int TH>
+__global__ __launch_bounds__(TH) void paged_extend_kernel(PagedDev p, const int32_t *__restrict__ n_new,
                                                                      StepDev st, int32_t *lens_out,
                                                                      int32_t *n_free_out) {
     __shared__ unsigned long long s_scan[17];
-    __shared__ long s_sum[17];
-    __shared__ int s_tok[kPagedThreads + 1], s_pg[kPagedThreads + 1], s_len[kPagedThreads];
+    __shared__ long s_sum[17 * 3];
+    __shared__ int s_tok[TH + 1], s_pg[TH + 1], s_len[TH];
     const int tid = threadIdx.x, page = 1 << p.page_shift;
     const long cap = (long)p.max_pages << p.page_shift;
     const int n_free = *p.n_free;
 
     // does the step fit? (totals in 64 bits: counts are not trusted yet)
     long tokens = 0, pages = 0, bad = (n_free < 0 || n_free > p.n_pages), over = 0;
-    for (int r = tid; r < p.n_requests; r += kPagedThreads) {
+    for (int r = tid; r < p.n_requests; r += TH) {
         const long len = p.lens[r], n = n_new[r];
         if (len < 0 || n < 0 || len > cap) {
             bad = 1;
@@ -102,9 +110,10 @@ __global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p,
         tokens += n;
         pages += ((len + n + page - 1) >> p.page_shift) - ((len + page - 1) >> p.page_shift);
     }
-    tokens = wg_sum(tokens, s_sum);
-    pages = wg_sum(pages, s_sum);
-    const long flags = wg_sum(bad | (over << 32), s_sum);
+    long sums[3] = {tokens, pages, bad | (over << 32)};
+    wg_sums(sums, s_sum);
+    tokens = sums[0], pages = sums[1];
+    const long flags = sums[2];
     const int status = (flags & 0xFFFFFFFFl) ? JK_PAGED_BAD_LENGTH
                        : (flags >> 32) || tokens > st.max_tokens ? JK_PAGED_TOO_LONG
                        : pages > n_free                          ? JK_PAGED_NO_PAGES
@@ -114,19 +123,19 @@ __global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p,
         *n_free_out = status == JK_PAGED_OK ? n_free - (int)pages : n_free;
     }
     if (status != JK_PAGED_OK) {
-        for (int r = tid; r < p.n_requests; r += kPagedThreads) {
+        for (int r = tid; r < p.n_requests; r += TH) {
             st.q_start[r] = 0;
             if (lens_out != p.lens) lens_out[r] = p.lens[r];
         }
         if (tid == 0) st.q_start[p.n_requests] = 0;
         if constexpr (FILL)
-            for (int t = tid; t < st.max_tokens; t += kPagedThreads) write_token(st, t, -1, -1, -1);
+            for (int t = tid; t < st.max_tokens; t += TH) write_token(st, t, -1, -1, -1);
         return;
     }
 
     unsigned long long carry = 0;  // tokens (low word) and pages (high word) of the requests before this pass
-    for (int r0 = 0; r0 < p.n_requests; r0 += kPagedThreads) {
-        const int r = r0 + tid, nr = min(kPagedThreads, p.n_requests - r0);
+    for (int r0 = 0; r0 < p.n_requests; r0 += TH) {
+        const int r = r0 + tid, nr = min(TH, p.n_requests - r0);
         const int len = r < p.n_requests ? p.lens[r] : 0, n = r < p.n_requests ? n_new[r] : 0;
         const int more = pages_of(len + n, p.page_shift) - pages_of(len, p.page_shift);
         unsigned long long sum;
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p,
         __syncthreads();
         if (r < p.n_requests) lens_out[r] = len + n;
         // new pages, one a thread: entry m is page m - s_pg of its request, from the top of the stack down
-        for (int m = s_pg[0] + tid; m < s_pg[nr]; m += kPagedThreads) {
+        for (int m = s_pg[0] + tid; m < s_pg[nr]; m += TH) {
             const int i = owner_of(s_pg, nr, m);
             const int j = pages_of(s_len[i], p.page_shift) + m - s_pg[i];
             const int id = p.free_pages[n_free - 1 - m];
@@ -152,7 +161,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p,
             p.table[cell] = p.owned[cell] = page_ok(id, p.n_pages) ? id : -1;
         }
         if constexpr (FILL) {
-            for (int t = s_tok[0] + tid; t < s_tok[nr]; t += kPagedThreads) {
+            for (int t = s_tok[0] + tid; t < s_tok[nr]; t += TH) {
                 const int i = owner_of(s_tok, nr, t), held = pages_of(s_len[i], p.page_shift);
                 const int pos = s_len[i] + t - s_tok[i], j = pos >> p.page_shift;
                 const int id = j < held ? p.table[(size_t)(r0 + i) * p.max_pages + j]
@@ -166,7 +175,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_extend_kernel(PagedDev p,
     const int total = (int)(uint32_t)carry;
     if (tid == 0) st.q_start[p.n_requests] = total;
     if constexpr (FILL)
-        for (int t = total + tid; t < st.max_tokens; t += kPagedThreads) write_token(st, t, -1, -1, -1);
+        for (int t = total + tid; t < st.max_tokens; t += TH) write_token(st, t, -1, -1, -1);
 }
 
 // Numbers the tokens of a planned step from q_start, the new lengths and the table.
@@ -250,10 +259,14 @@ __device__ __forceinline__ int parent_row(const int32_t *parent, int row, int wi
 // First half of the reordering, in one workgroup: takes a page for each row that has none to go on
 // filling, and writes the new lengths. Passes hold whole groups, so that in place a group's lengths are
 // all read before one of them is written.
-__global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(PagedDev p,
-                                                                           const int32_t *__restrict__ parent,
-                                                                           int width, int32_t *status,
-                                                                           int32_t *lens_out) {
+// TABLE: it also writes the tables, of few cells (one launch instead of two).
+template <int MW>
+__device__ __forceinline__ void reorder_column(const PagedDev &p, const int32_t *parent, int width, bool ok,
+                                               const int32_t *lens, int32_t *table_out, int g, int j);
+template <bool TABLE, int MW>
+__global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(PagedDev p, const int32_t *parent, int width,
+                                                                           int32_t *status, int32_t *lens_out,
+                                                                           int32_t *table_out) {
     __shared__ unsigned long long s_scan[17];
     __shared__ long s_sum[17];
     const int tid = threadIdx.x, mask = (1 << p.page_shift) - 1;
@@ -273,19 +286,22 @@ __global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(Paged
         if (!page_ok(own, p.n_pages) || own != p.table[(size_t)from * p.max_pages + j]) *flags |= 1l << 32;
         return !page_ok(p.owned[(size_t)row * p.max_pages + j], p.n_pages);
     };
-    long need = 0, flags = 0;
-    int len;
-    for (int row = tid; row < p.n_requests; row += kPagedThreads) {
+    // sums: rows that take a page, threads that met a bad length (from bit 32) and a page not owned (from bit 48)
+    long found[1] = {0};
+    int len = 0;
+    bool takes = false;
+    const bool one = p.n_requests <= per;  // (one pass: what it finds is kept)
+    for (int row = tid; row < p.n_requests; row += one ? p.n_requests : kPagedThreads) {
         long f = 0;
-        need += look(row, &len, &f);
-        flags |= f;
+        takes = look(row, &len, &f);
+        found[0] = ((found[0] | ((f & 1) << 32) | ((f >> 32) << 48))) + takes;
     }
-    need = wg_sum(need, s_sum);
-    flags = wg_sum(flags, s_sum);
-    const int st = (flags & 0xFFFFFFFFl) || n_free < 0 || n_free > p.n_pages ? JK_PAGED_BAD_LENGTH
-                   : flags                                                  ? JK_PAGED_NOT_OWNED
-                   : need > n_free                                          ? JK_PAGED_NO_PAGES
-                                                                            : JK_PAGED_OK;
+    wg_sums(found, s_sum);
+    const long need = found[0] & 0xFFFFFFFFl;
+    const int st = ((found[0] >> 32) & 0xFFFF) || n_free < 0 || n_free > p.n_pages ? JK_PAGED_BAD_LENGTH
+                   : found[0] >> 48                                                ? JK_PAGED_NOT_OWNED
+                   : need > n_free                                                 ? JK_PAGED_NO_PAGES
+                                                                                   : JK_PAGED_OK;
     __syncthreads();  // (every thread has read n_free)
     if (tid == 0) {
         *status = st;
@@ -294,16 +310,19 @@ __global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(Paged
     if (st != JK_PAGED_OK) {
         if (lens_out != p.lens)
             for (int row = tid; row < p.n_requests; row += kPagedThreads) lens_out[row] = p.lens[row];
+        if (TABLE && table_out != p.table)
+            for (int i = tid; i < p.n_requests * p.max_pages; i += kPagedThreads) table_out[i] = p.table[i];
         return;
     }
     int taken = 0;
     for (int r0 = 0; r0 < p.n_requests; r0 += per) {
         const int row = r0 + tid;
         const bool live = tid < per && row < p.n_requests;
-        bool takes = false;
-        long f = 0;
-        len = 0;
-        if (live) takes = look(row, &len, &f);
+        if (!one) {
+            long f = 0;
+            takes = live && look(row, &len, &f);
+        }
+        takes = takes && live;
         unsigned long long sum;
         const int at = taken + (int)wg_scan((unsigned long long)takes, s_scan, &sum);  // (a barrier: all have read)
         if (takes) {
@@ -313,20 +332,20 @@ __global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(Paged
         if (live) lens_out[row] = len;
         taken += (int)sum;
     }
+    if constexpr (TABLE) {
+        __syncthreads();
+        const int groups = p.n_requests / width;
+        for (int i = tid; i < groups * p.max_pages; i += kPagedThreads)
+            reorder_column<MW>(p, parent, width, true, lens_out, table_out, i / p.max_pages, i % p.max_pages);
+    }
 }
 
 // Second half: one thread takes one column of a group's rows, reads all of them and then writes them, so the
 // permutation can be in place. lens: the new lengths.
 template <int MW>
-__global__ __launch_bounds__(256) void paged_reorder_table_kernel(PagedDev p, const int32_t *__restrict__ parent,
-                                                                  int width, const int32_t *__restrict__ status,
-                                                                  const int32_t *__restrict__ lens, int32_t *table_out,
-                                                                  int col_blocks) {
-    const int g = blockIdx.x / col_blocks, j = (blockIdx.x % col_blocks) * 256 + threadIdx.x;
-    if (j >= p.max_pages) return;
+__device__ __forceinline__ void reorder_column(const PagedDev &p, const int32_t *parent, int width, bool ok,
+                                               const int32_t *lens, int32_t *table_out, int g, int j) {
     const int row0 = g * width, mask = (1 << p.page_shift) - 1;
-    const bool ok = *status == JK_PAGED_OK;
-    if (!ok && table_out == p.table) return;
     int v[MW];
 #pragma unroll
     for (int b = 0; b < MW; ++b) {
@@ -341,6 +360,16 @@ __global__ __launch_bounds__(256) void paged_reorder_table_kernel(PagedDev p, co
         if (b >= width) break;
         table_out[(size_t)(row0 + b) * p.max_pages + j] = v[b];
     }
+}
+template <int MW>
+__global__ __launch_bounds__(256) void paged_reorder_table_kernel(PagedDev p, const int32_t *__restrict__ parent,
+                                                                  int width, const int32_t *__restrict__ status,
+                                                                  const int32_t *lens, int32_t *table_out,
+                                                                  int col_blocks) {
+    const int j = (blockIdx.x % col_blocks) * 256 + threadIdx.x;
+    const bool ok = *status == JK_PAGED_OK;
+    if (j >= p.max_pages || (!ok && table_out == p.table)) return;
+    reorder_column<MW>(p, parent, width, ok, lens, table_out, blockIdx.x / col_blocks, j);
 }
 
 // Moves the pages that are being filled: one thread takes 16 bytes of one head's rows of every
@@ -448,11 +477,16 @@ jk_status jk_paged_extend(jk_stream s, const jk_paged *p, const int32_t *n_new, 
     int32_t *lo = lens_out ? lens_out : p->lens, *fo = n_free_out ? n_free_out : p->n_free;
     // one workgroup numbers up to this many tokens itself
     if (st->max_tokens <= 2 * kPagedThreads) {
-        hipLaunchKernelGGL(paged_extend_kernel<true>, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, n_new, sd, lo,
-                           fo);
+        if (p->n_requests <= 256 && st->max_tokens <= 512)  // (few waves to a barrier)
+            hipLaunchKernelGGL((paged_extend_kernel<true, 256>), dim3(1), dim3(256), 0, (hipStream_t)s, d, n_new, sd, lo,
+                               fo);
+        else
+            hipLaunchKernelGGL((paged_extend_kernel<true, kPagedThreads>), dim3(1), dim3(kPagedThreads), 0,
+                               (hipStream_t)s, d, n_new, sd, lo, fo);
         return check_launch("paged_extend_kernel");
     }
-    hipLaunchKernelGGL(paged_extend_kernel<false>, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, n_new, sd, lo, fo);
+    hipLaunchKernelGGL((paged_extend_kernel<false, kPagedThreads>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d,
+                       n_new, sd, lo, fo);
     JK_TRY(check_launch("paged_extend_kernel"));
     hipLaunchKernelGGL(paged_fill_kernel, dim3((unsigned)((st->max_tokens + kFillThreads - 1) / kFillThreads)),
                        dim3(kFillThreads), 0, (hipStream_t)s, d, sd, lo);
@@ -480,16 +514,26 @@ jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent
     const size_t col_blocks = (p->max_pages + 255) / 256, groups = p->n_requests / width;
     if (col_blocks * groups > kMaxBlocks)
         return fail(JK_TENSOR_BOUNDS, "paged_reorder: a table of %zu x %zu is too large", p->n_requests, p->max_pages);
-    hipLaunchKernelGGL(paged_reorder_plan_kernel, dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, parent, (int)width,
-                       status, lo);
+    const int w = (int)width;
+    if (groups * p->max_pages <= (size_t)4 * kPagedThreads) {
+        if (width <= 8)
+            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 8>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d,
+                               parent, w, status, lo, to);
+        else
+            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 32>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d,
+                               parent, w, status, lo, to);
+        return check_launch("paged_reorder_plan_kernel");
+    }
+    hipLaunchKernelGGL((paged_reorder_plan_kernel<false, 8>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, parent,
+                       w, status, lo, to);
     JK_TRY(check_launch("paged_reorder_plan_kernel"));
     const dim3 grid((unsigned)(col_blocks * groups));
     if (width <= 8)
-        hipLaunchKernelGGL(paged_reorder_table_kernel<8>, grid, dim3(256), 0, (hipStream_t)s, d, parent, (int)width,
-                           status, lo, to, (int)col_blocks);
+        hipLaunchKernelGGL(paged_reorder_table_kernel<8>, grid, dim3(256), 0, (hipStream_t)s, d, parent, w, status, lo,
+                           to, (int)col_blocks);
     else
-        hipLaunchKernelGGL(paged_reorder_table_kernel<32>, grid, dim3(256), 0, (hipStream_t)s, d, parent, (int)width,
-                           status, lo, to, (int)col_blocks);
+        hipLaunchKernelGGL(paged_reorder_table_kernel<32>, grid, dim3(256), 0, (hipStream_t)s, d, parent, w, status, lo,
+                           to, (int)col_blocks);
     return check_launch("paged_reorder_table_kernel");
 }
 

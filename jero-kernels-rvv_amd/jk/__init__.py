@@ -123,6 +123,15 @@ class WeightLayoutC(C.Structure):
         return count * self.scale_groups * 8
 
 
+# The entry points of a serving step, by their argument types.
+_STEP_CALLS = {
+    "jk_paged_reset": [_vp, _vp], "jk_paged_extend": [_vp, _vp, _vp, _vp, _vp, _vp],
+    "jk_paged_release": [_vp, _vp, _vp], "jk_paged_reorder": [_vp, _vp, _vp, _sz, _vp, _vp, _vp],
+    "jk_kv_append_q8": [_vp, _vp, _vp, _vp, C.c_int, _sz, _sz, _sz, _vp],
+    "jk_kv_read_q8": [_vp, _vp, _vp, _sz, C.c_int, _vp, _vp],
+    "jk_kv_reorder_q8": [_vp, _vp, _vp, _vp, _sz, _vp], "jk_attn_q8": [_vp, _vp, _vp, _vp, _sz],
+    "jk_beam_select": [_vp, _vp, _vp, _sz],
+}
 _lib_handle = None
 
 
@@ -137,6 +146,9 @@ def lib() -> C.CDLL:
         h.jk_act_q8_bytes.restype = _sz
         h.jk_attn_q8_workspace_bytes.restype = _sz
         h.jk_beam_workspace_bytes.restype = _sz
+        # (with prototypes these take plain ints: a decode step calls them for every layer)
+        for name, types in _STEP_CALLS.items():
+            getattr(h, name).argtypes = types
         h.jk_act_q8_bytes.argtypes = [_sz, _sz]
         _lib_handle = h
     return _lib_handle
@@ -888,24 +900,24 @@ def paged_step(q_start, slots, positions, requests, status) -> PagedStepC:
 
 def dev_paged_reset(p: PagedC, stream=None):
     """jk_paged_reset: empty requests, all pages free."""
-    _check(lib().jk_paged_reset(_vp(stream or 0), C.byref(p)))
+    _check(lib().jk_paged_reset(stream, C.byref(p)))
 
 
 def dev_paged_extend(p: PagedC, n_new, step: PagedStepC, lens_out=None, n_free_out=None, stream=None):
     """jk_paged_extend: n_new[r] more tokens for each request; pages, slots and positions of the step's tokens."""
-    _check(lib().jk_paged_extend(_vp(stream or 0), C.byref(p), _vp(_ptr(n_new)), C.byref(step), _vp(_ptr(lens_out)),
-                                 _vp(_ptr(n_free_out))))
+    _check(lib().jk_paged_extend(stream, C.byref(p), _ptr(n_new), C.byref(step), _ptr(lens_out),
+                                 _ptr(n_free_out)))
 
 
 def dev_paged_release(p: PagedC, ended, stream=None):
     """jk_paged_release: the pages of the requests with ended[r] != 0 back on the stack."""
-    _check(lib().jk_paged_release(_vp(stream or 0), C.byref(p), _vp(_ptr(ended))))
+    _check(lib().jk_paged_release(stream, C.byref(p), _ptr(ended)))
 
 
 def dev_paged_reorder(p: PagedC, parent, width: int, status, lens_out=None, table_out=None, stream=None):
     """jk_paged_reorder: row r of each group of `width` goes on from row parent[r]."""
-    _check(lib().jk_paged_reorder(_vp(stream or 0), C.byref(p), _vp(_ptr(parent)), _sz(width), _vp(_ptr(status)),
-                                  _vp(_ptr(lens_out)), _vp(_ptr(table_out))))
+    _check(lib().jk_paged_reorder(stream, C.byref(p), _ptr(parent), width, _ptr(status),
+                                  _ptr(lens_out), _ptr(table_out)))
 
 
 def kv_q8(k, v, k_scale, v_scale) -> KvQ8C:
@@ -927,8 +939,8 @@ def dev_kv_append_q8(c: KvQ8C, k, v, slots, stream=None):
     if tuple(k.shape[1:]) != (c.n_kv, c.head_dim) or slots.numel() != k.shape[0]:
         raise TensorBoundsError("keys of the cache's heads and one slot a token are needed")
     _i32(slots)
-    _check(lib().jk_kv_append_q8(_vp(stream or 0), C.byref(c), _vp(_ptr(k)), _vp(_ptr(v)), C.c_int(_dtype_of(k)),
-                                 _sz(k.shape[0]), _sz(st), _sz(sh), _vp(_ptr(slots))))
+    _check(lib().jk_kv_append_q8(stream, C.byref(c), _ptr(k), _ptr(v), _dtype_of(k),
+                                 k.shape[0], st, sh, _ptr(slots)))
 
 
 def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
@@ -938,14 +950,14 @@ def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
     for x in outs:
         if not x.is_contiguous() or x.numel() != slots.numel() * c.n_kv * c.head_dim or x.dtype != outs[0].dtype:
             raise TensorBoundsError("outputs need packed tensors [slots][kv heads][head_dim] of one type")
-    _check(lib().jk_kv_read_q8(_vp(stream or 0), C.byref(c), _vp(_ptr(slots)), _sz(slots.numel()),
-                               C.c_int(_dtype_of(outs[0]) if outs else F32), _vp(_ptr(k_out)), _vp(_ptr(v_out))))
+    _check(lib().jk_kv_read_q8(stream, C.byref(c), _ptr(slots), slots.numel(),
+                               _dtype_of(outs[0]) if outs else F32, _ptr(k_out), _ptr(v_out)))
 
 
 def dev_kv_reorder_q8(c: KvQ8C, p: PagedC, parent, width: int, status, stream=None):
     """jk_kv_reorder_q8: the cache's part of dev_paged_reorder, after it, for each layer."""
-    _check(lib().jk_kv_reorder_q8(_vp(stream or 0), C.byref(c), C.byref(p), _vp(_ptr(parent)), _sz(width),
-                                  _vp(_ptr(status))))
+    _check(lib().jk_kv_reorder_q8(stream, C.byref(c), C.byref(p), _ptr(parent), width,
+                                  _ptr(status)))
 
 
 def attn_q8_args(q, out, q_start, lens, table, max_new: int, max_len: int, scale: float, window: int = 0) -> AttnQ8ArgsC:
@@ -969,7 +981,7 @@ def attn_q8_workspace_bytes(c: KvQ8C, a: AttnQ8ArgsC) -> int:
 
 def dev_attn_q8(c: KvQ8C, a: AttnQ8ArgsC, ws=None, stream=None, ws_bytes=None):
     """jk_attn_q8: causal attention of the step's queries over the paged 8-bit cache."""
-    _check(lib().jk_attn_q8(_vp(stream or 0), C.byref(c), C.byref(a), _vp(_ptr(ws)), _sz(_ws_bytes(ws, ws_bytes))))
+    _check(lib().jk_attn_q8(stream, C.byref(c), C.byref(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
 
 
 def beam_args(logits, scores, done, scores_out, parents, tokens, done_out=None, eos: int = -1) -> BeamArgsC:
@@ -997,7 +1009,7 @@ def beam_workspace_bytes(a: BeamArgsC) -> int:
 
 def dev_beam_select(a: BeamArgsC, ws, stream=None, ws_bytes=None):
     """jk_beam_select: the width best continuations of each group's hypotheses."""
-    _check(lib().jk_beam_select(_vp(stream or 0), C.byref(a), _vp(_ptr(ws)), _sz(_ws_bytes(ws, ws_bytes))))
+    _check(lib().jk_beam_select(stream, C.byref(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
 
 
 def dev_measure_stream_read(buf, nbytes, sink, stream=None):
