@@ -864,7 +864,8 @@ def _strides(x) -> tuple[int, int]:
     """Token and head strides of a [tokens][heads][head_dim] tensor whose last dimension is packed."""
     if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
         raise TensorBoundsError("a [tokens][heads][head_dim] tensor with a packed last dimension is needed")
-    return x.stride(0), x.stride(1)
+    # (of a dimension of one element torch leaves any stride: 0, packed)
+    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
 
 
 def _held(struct, *tensors):
