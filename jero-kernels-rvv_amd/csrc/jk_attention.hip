@@ -15,7 +15,7 @@ namespace jk {
 // and nothing goes through LDS.
 // PARTS: f16 parts that f32 queries and probabilities are split into.
 template <typename T, int HDP, int PARTS>
-__global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
+__global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(AttnDev a) {
     constexpr int KJ = HDP / 64, NT = HDP / 16, VW = HDP / 64;  // VW: dwords of a value row that a lane loads
     __shared__ float s_ml[4][16][3];
     __shared__ float s_o[4][16][HDP + 4];
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
     f32x4 o[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f32x4{0, 0, 0, 0};
-    float m = kNegInf, lsum = 0.0f, vref = 0.0f;
+    float m = kNegInf, lsum = 0.0f, vref = 0.0f, per = 0.0f;  // per: kWeight / vref, 0 while all values are
 
     // Byte offsets of this lane's loads inside 16 tokens' rows. Channels past the head dimension are read
     // from the row's start: queries are 0 there, and outputs are not stored.
@@ -115,13 +115,16 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
         }
         top = max_rows(top);
         const int e2 = range_shift(top);
-        to_score = ldexpf(a.scale_log2, -e2);
+        to_score = ldexpf(fabsf(a.scale_log2), -e2);  // (its sign goes to the queries)
 #pragma unroll
         for (int j = 0; j < 2 * KJ; ++j) {
             float y[8];
             f16x8 part[PARTS];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[j / 2][8 * (j % 2) + e], e2);
+            for (int e = 0; e < 8; ++e) {
+                const float q = x[j / 2][8 * (j % 2) + e];
+                y[e] = ldexpf(a.scale_log2 < 0.0f ? -q : q, e2);
+            }
             split_f16<PARTS>(y, part);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) qf[p][j] = part[p];
@@ -131,7 +134,7 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
 
     const int pos_lo = rq.len - rq.count + c0 / a.grp, pos_hi = rq.len - rq.count + (min(c0 + 16, cols) - 1) / a.grp;
     auto use = [&](int t0, Tile &x) {
-        float s[8], top = kNegInf;
+        float s[8], f[2], vs[2], top = kNegInf;
         // (tiles that every column sees whole need no comparisons)
         const bool whole = x.there[0] && x.there[1] && t0 + 31 <= pos_lo && pos_hi - t0 < a.window;
 #pragma unroll
@@ -146,39 +149,51 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[p][2 * j + 1], acc, 0, 0, 0);
                 }
             }
-            const float f = x.ks[u] * to_score;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * u + i] = acc[i] * f;
+            for (int i = 0; i < 4; ++i) s[4 * u + i] = acc[i];
+            vs[u] = x.there[u] ? x.vs[u] : 0.0f;
         }
         if (!whole) {
+            asm("" : "+v"(s[0]));  // (keeps the branch: few tiles need this, and selects would cost every tile)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
                 if (!(x.there[i / 4] && t <= pos && pos - t < a.window)) s[i] = kNegInf;
             }
         }
+        // scores are s * f, f one number a page and positive (0 becomes next to nothing: an unseen -inf stays one)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i]);
-        const float m_new = fmaxf(m, max_rows(top)), m_use = m_new == kNegInf ? 0.0f : m_new;
-        const float vs[2] = {x.there[0] ? x.vs[0] : 0.0f, x.there[1] ? x.vs[1] : 0.0f};
-        const float vref_new = fmaxf(vref, fmaxf(vs[0], vs[1])), per = vref_new > 0.0f ? 1.0f / vref_new : 0.0f;
-        const float fade = exp2_fast(m - m_use), fade_o = vref == vref_new ? fade : fade * (vref * per);
-        const float vw[2] = {vs[0] * (per * kWeightScale), vs[1] * (per * kWeightScale)};
-        lsum *= fade;
-        f16x8 wf[PARTS];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float p = exp2_fast(s[i] - m_use);  // (unseen: 2^-inf = 0)
-            lsum += p;
-            s[i] = p * vw[i / 4];
+        for (int u = 0; u < 2; ++u) {
+            f[u] = x.ks[u] * to_score;
+            f[u] = f[u] < 1e-37f ? 1e-37f : f[u];
+            top = fmaxf(top, fmaxf(fmaxf(s[4 * u], s[4 * u + 1]), fmaxf(s[4 * u + 2], s[4 * u + 3])) * f[u]);
         }
-        split_f16<PARTS>(s, wf);
-        m = m_new;
-        vref = vref_new;
-        if (__any(fade_o != 1.0f)) {
+        const bool vmove = fmaxf(vs[0], vs[1]) > vref * kSlackV;
+        if (vmove || __any(top > m + kSlack)) {
+            top = max_rows(top);
+            const float m_new = top > m + kSlack ? top : m, vref_new = vmove ? fmaxf(vs[0], vs[1]) : vref;
+            // (the first reference of a column comes from nothing: nothing is kept)
+            const float fade = m_new == m ? 1.0f : exp2_fast(m - m_new), fade_o = vmove ? fade * (vref / vref_new) : fade;
+            m = m_new;
+            vref = vref_new;
+            per = kWeight / vref;
+            lsum *= fade;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= fade_o;
         }
+        const float m_use = m == kNegInf ? 0.0f : m;
+        f16x8 wf[PARTS];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float vw = vs[u] * per;
+#pragma unroll
+            for (int i = 4 * u; i < 4 * u + 4; ++i) {
+                const float p = exp2_fast(__builtin_fmaf(s[i], f[u], -m_use));  // (unseen: 2^-inf = 0)
+                lsum += p;
+                s[i] = p * vw;
+            }
+        }
+        split_f16<PARTS>(s, wf);
 #pragma unroll
         for (int e = 0; e < VW; ++e)
 #pragma unroll
@@ -218,7 +233,7 @@ __global__ __launch_bounds__(256) void attn_q8_rows_kernel(AttnDev a) {
     for (int i = 0; i < 4; ++i) m_all = fmaxf(m_all, s_ml[i][n][0]);
     const float m_use = m_all == kNegInf ? 0.0f : m_all;
     // (NaN scores leave m at -inf but make the sum NaN: it must not be multiplied away)
-    const float mine = m == kNegInf ? (__builtin_isnan(lsum) ? lsum : 0.0f) : exp2_fast(m - m_use) * vref * (kCodeScale / kWeightScale);
+    const float mine = m == kNegInf ? (__builtin_isnan(lsum) ? lsum : 0.0f) : exp2_fast(m - m_use) * vref * (kCodeScale / kWeight);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll

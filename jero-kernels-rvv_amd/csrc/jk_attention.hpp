@@ -8,7 +8,7 @@
 //   s_j = scale q.k_j,  p_j = exp(s_j - m),  l = sum p_j,  o = sum p_j v_j / l
 // with k_j = ks * codes and v_j = vs * codes, ks and vs one number per page and head. The products run on f16
 // matrix instructions: codes are exact in f16, ks multiplies the finished score, and vs joins the
-// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j <= 1 whatever the values' size (held times 2^14); o is
+// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j stays in f16's range whatever the values' size; o is
 // rescaled by r like by m. Scores are computed transposed (rows = tokens), so a lane that holds a column's
 // scores of four consecutive tokens holds them just as the second product's operand wants them: the order
 // of the tokens inside a matrix instruction is free as long as both of its operands agree on it.
@@ -24,9 +24,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kCodeScale = 512.0f;  // a code becomes code / 512 in f16 (code_pair)
-// Queries and weights are held in f16 with their largest values near 2^14, so that what is 2^-28 of those is still a
-// normal number, and the low parts of f32 ones keep their bits: weights are p_j vs / r times this.
-constexpr float kWeightScale = 16384.0f;
+// Queries are held in f16 with their row's largest value near 2^14, so that what is 2^-28 of it is still a normal number and
+// the low parts of f32 ones keep their bits.
+// The maximum that weights are taken against is a reference that moves only when a tile's scores pass it by kSlack powers of
+// two, and so is the largest value scale, by a factor of kSlackV: almost no tile has to rescale the outputs, or to find
+// its maximum across lanes. Weights are p_j vs / r times kWeight: at most 16 * 2^8 * 8 = 2^15, which f16 holds, and what is
+// 2^-18 of the reference is still a normal number.
+constexpr float kSlack = 8.0f, kSlackV = 8.0f, kWeight = 16.0f;
 
 struct AttnDev {
     const void *q;

@@ -9,9 +9,6 @@ namespace jk {
 //      8 channels of token lane % 32.
 //   V: [channel][64 tokens], the tokens of each 16 ordered 0-3, 8-11, 4-7, 12-15: a lane of the second product (rows =
 //      channels) reads the 8 tokens whose scores the first one left in that half of the wave.
-// The running maximum is a reference that moves only when a tile's scores pass it by 2^kSlack (and so is the largest value
-// scale, by kSlackV): weights may be that much larger than 1, which f16 holds, and almost no tile has to rescale the outputs.
-constexpr float kSlack = 8.0f, kSlackV = 8.0f, kPromptWeight = 16.0f;  // 16 * 2^8 * 8 = 2^15
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // PG: pages that a tile can lie in: 1 (pages of 64 tokens or more), 2 or 4.
@@ -210,9 +207,9 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             whole = whole && pages.head[i] >= 0;
         }
         const bool vmove = vtop > vref * kSlackV;
-        const float vref_new = vmove ? vtop : vref, per = vref_new > 0.0f ? kPromptWeight / vref_new : 0.0f;
+        const float vref_new = vmove ? vtop : vref, per = vref_new > 0.0f ? kWeight / vref_new : 0.0f;
         if (!whole) {
-            asm volatile("");  // (a branch: few tiles need this, and selects would cost every tile)
+            asm("" : "+v"(s[0][0].v[0]));  // (keeps the branch: few tiles need this, and selects would cost every tile)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -324,7 +321,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         const float lall = sum_halves(lsum[c]);
         if (col >= cols) continue;
         const int token = rq.first + col / a.grp, head = h * a.grp + col % a.grp;
-        const float to_out = vref * (kCodeScale / kPromptWeight);
+        const float to_out = vref * (kCodeScale / kWeight);
         const float inv = sp.active > 1 ? to_out : lall == 0.0f ? 0.0f : to_out / lall;
         const size_t at = ((size_t)token * a.n_heads + head) * a.pitch + split;
         typename T::raw *out = static_cast<typename T::raw *>(a.out) + (size_t)token * a.ot + (size_t)head * a.oh;
