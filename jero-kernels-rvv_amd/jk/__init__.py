@@ -822,7 +822,9 @@ def op_counts() -> tuple[int, int]:
 # ------------------------------------------- paged 8-bit attention cache, beam search
 F32, F16, BF16 = 0, 1, 30  # jk_dtype
 PAGED_OK, PAGED_NO_PAGES, PAGED_TOO_LONG, PAGED_BAD_LENGTH, PAGED_NOT_OWNED = 0, 1, 2, 3, 4
-_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "float32": F32, "float16": F16}
+_I32 = -1  # (of the index arrays; not a jk_dtype)
+_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int32": _I32}
+_dtype_codes = {}  # the same by dtype object, filled as they are met (a name costs more than a call's other checks)
 
 
 class PagedC(C.Structure):
@@ -853,19 +855,29 @@ class BeamArgsC(C.Structure):
                 ("parents", _vp), ("tokens", _vp), ("done_out", _vp)]
 
 
+def _code_of(x):
+    t = x.dtype
+    if t not in _dtype_codes:
+        _dtype_codes[t] = _DTYPES.get(str(t))
+    return _dtype_codes[t]
+
+
 def _dtype_of(x) -> int:
-    t = _DTYPES.get(str(x.dtype))
-    if t is None:
+    t = _code_of(x)
+    if t is None or t == _I32:
         raise CapabilityMismatch(f"element type {x.dtype}: float32, float16 or bfloat16")
     return t
 
 
 def _strides(x) -> tuple[int, int]:
     """Token and head strides of a [tokens][heads][head_dim] tensor whose last dimension is packed."""
-    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or (shape[2] > 1 and stride[2] != 1):
         raise TensorBoundsError("a [tokens][heads][head_dim] tensor with a packed last dimension is needed")
+    if (shape[0] > 1 and stride[0] == 0) or (shape[1] > 1 and stride[1] == 0):
+        raise TensorBoundsError("an expanded tensor (a stride of 0 means packed to the library) has to be made contiguous")
     # (of a dimension of one element torch leaves any stride: 0, packed)
-    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+    return stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
 
 def _held(struct, *tensors):
@@ -876,7 +888,7 @@ def _held(struct, *tensors):
 
 def _i32(*tensors):
     for x in tensors:
-        if x is not None and (str(x.dtype) != "torch.int32" or not x.is_contiguous()):
+        if x is not None and (_code_of(x) != _I32 or not x.is_contiguous()):
             raise TensorBoundsError("a packed int32 tensor is needed")
 
 
@@ -935,13 +947,13 @@ def kv_q8(k, v, k_scale, v_scale) -> KvQ8C:
 def dev_kv_append_q8(c: KvQ8C, k, v, slots, stream=None):
     """jk_kv_append_q8: k and v [tokens][kv heads][head_dim] (the same strides) into their slots."""
     st, sh = _strides(k)
+    n, kv, hd = k.shape
     if _strides(v) != (st, sh) or v.shape != k.shape or v.dtype != k.dtype:
         raise TensorBoundsError("keys and values need the same shape, strides and type")
-    if tuple(k.shape[1:]) != (c.n_kv, c.head_dim) or slots.numel() != k.shape[0]:
+    if kv != c.n_kv or hd != c.head_dim or slots.numel() != n:
         raise TensorBoundsError("keys of the cache's heads and one slot a token are needed")
     _i32(slots)
-    _check(lib().jk_kv_append_q8(stream, C.byref(c), _ptr(k), _ptr(v), _dtype_of(k),
-                                 k.shape[0], st, sh, _ptr(slots)))
+    _check(lib().jk_kv_append_q8(stream, C.byref(c), k.data_ptr(), v.data_ptr(), _dtype_of(k), n, st, sh, _ptr(slots)))
 
 
 def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
@@ -998,6 +1010,8 @@ def beam_args(logits, scores, done, scores_out, parents, tokens, done_out=None, 
     if logits.dim() != 2 or logits.shape[0] != groups * width or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise TensorBoundsError("logits need one packed row a hypothesis")
     stride = logits.stride(0) if logits.shape[0] > 1 else 0
+    if logits.shape[0] > 1 and stride == 0:
+        raise TensorBoundsError("expanded logits (a stride of 0 means packed to the library) have to be made contiguous")
     return _held(BeamArgsC(_ptr(logits), _dtype_of(logits), groups, width, logits.shape[1], stride, _ptr(scores),
                            _ptr(done), eos, _ptr(scores_out), _ptr(parents), _ptr(tokens), _ptr(done_out)),
                  logits, scores, done, scores_out, parents, tokens, done_out)
