@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
         }
         top = max_rows(top);
         const int e2 = range_shift(top);
-        to_score = ldexpf(fabsf(a.scale_log2), -e2);  // (its sign goes to the queries)
+        to_score = ldexpf(fabsf(a.scale_log2), kCodeShift - e2);  // (its sign goes to the queries)
 #pragma unroll
         for (int j = 0; j < 2 * KJ; ++j) {
             float y[8];
@@ -356,8 +356,10 @@ static jk_status attn_check(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
 // there are two tiles a CU to level out their lengths, else 128 (two a CU: 64 us for 2048 tokens against 96).
 // Where there are fewer tiles than places, their keys are cut into chunks of one size for the whole call, a place's share of the work,
 // so that the last ones are not left with a long request or with a prompt's last tiles, which see the most keys. Up to kWholeLen
-// keys are not cut in the rows kernel: the second launch costs more than it saves (three requests of up to 700 keys 9 us whole, 13
-// in two; one of 1000 12.4 and 14; of 2000 17.5 and 14).
+// keys are not cut: the second launch costs more than it saves (decode step of three requests of up to 700 keys 9 us whole, 13
+// in two; one of 1000 12.4 and 14; of 2000 17.5 and 14. A prompt of 1024 tokens 34 us whole and 50 in two; two of 700 after 300
+// 39 and 75; 512 tokens after 500 33 and 38, but of 256 channels 64 and 56). Longer ones go down to kMinPromptChunk keys (512
+// tokens after 2000 52 us, with 1024 keys at least 64; 1024 after 1000 83 and 73).
 constexpr size_t kFewCols = 1024, kFewColsF32 = 2048, kMixedCols = 64, kMinChunk = 256, kMinPromptChunk = 512, kWholeLen = 1024;
 struct AttnPlan {
     size_t few_tiles, few_splits, few_chunk, many_cols, many_tiles, many_splits, many_chunk, few_cols, pitch;
@@ -369,7 +371,7 @@ static AttnPlan attn_plan(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
     size_t len = std::min(a->max_len, a->max_pages * c->page);
     if (a->window) len = std::min(len, a->window + new_tokens);
     auto cut = [&](size_t share, size_t least, size_t *splits, size_t *chunk) {
-        *chunk = std::max({share, least, (len + kMaxSplits - 1) / kMaxSplits});
+        *chunk = std::max({share, len <= kWholeLen ? kWholeLen : least, (len + kMaxSplits - 1) / kMaxSplits});
         *chunk = (*chunk + 127) / 128 * 128;
         *splits = std::max<size_t>(1, (len + *chunk - 1) / *chunk);
     };
@@ -378,7 +380,7 @@ static AttnPlan attn_plan(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
     p.few_splits = p.many_splits = p.few_chunk = p.many_chunk = 1;
     if (p.few_cols) {
         p.few_tiles = (std::min(cols, p.few_cols) + 15) / 16;
-        cut(heads * p.few_tiles * len / ncu, len <= kWholeLen ? kWholeLen : kMinChunk, &p.few_splits, &p.few_chunk);
+        cut(heads * p.few_tiles * len / ncu, kMinChunk, &p.few_splits, &p.few_chunk);
     }
     if (cols > p.few_cols) {
         p.many_cols = c->head_dim <= 128 && heads * ((cols + 255) / 256) >= 2 * ncu ? 256 : 128;
@@ -435,7 +437,7 @@ jk_status jk_attn_q8(jk_stream s, const jk_kv_q8 *c, const jk_attn_q8_args *a, v
     const size_t es = dtype_bytes(a->dtype);
     if ((uintptr_t)a->q % es || (uintptr_t)a->out % es)
         return fail(JK_TENSOR_BOUNDS, "attn_q8: queries and output must be aligned to their elements");
-    if (!std::isfinite(a->scale)) return fail(JK_TENSOR_BOUNDS, "attn_q8: scale %g", (double)a->scale);
+    if (!std::isfinite(a->scale * kLog2e)) return fail(JK_TENSOR_BOUNDS, "attn_q8: scale %g", (double)a->scale);
     AttnDev d{};
     d.q = a->q, d.out = a->out;
     d.qh = a->q_stride_head ? a->q_stride_head : c->head_dim, d.oh = a->out_stride_head ? a->out_stride_head : c->head_dim;
@@ -451,7 +453,7 @@ jk_status jk_attn_q8(jk_stream s, const jk_kv_q8 *c, const jk_attn_q8_args *a, v
     d.max_new = (int)std::min<size_t>(a->max_new, a->n_tokens);
     d.q_start = a->q_start, d.lens = a->lens, d.table = a->table;
     d.k = c->k, d.v = c->v, d.ks = c->k_scale, d.vs = c->v_scale;
-    d.scale_log2 = a->scale * 1.44269504088896340736f * kCodeScale;
+    d.scale_log2 = a->scale * kLog2e;
     d.window = a->window == 0 || a->window > (size_t)INT32_MAX ? INT32_MAX : (int)a->window;
     const AttnPlan plan = attn_plan(c, a);
     d.few_cols = (int)plan.few_cols, d.few_splits = (int)plan.few_splits, d.few_chunk = (int)plan.few_chunk;

@@ -23,7 +23,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kCodeScale = 512.0f;  // a code becomes code / 512 in f16 (code_pair)
+constexpr int kCodeShift = 9;  // a code becomes code / 2^9 in f16 (code_pair)
+constexpr float kCodeScale = 1 << kCodeShift;
+constexpr float kLog2e = 1.44269504088896340736f;
 // Queries are held in f16 with their row's largest value near 2^14, so that what is 2^-28 of it is still a normal number and
 // the low parts of f32 ones keep their bits.
 // The maximum that weights are taken against is a reference that moves only when a tile's scores pass it by kSlack powers of
@@ -41,7 +43,7 @@ struct AttnDev {
     const int32_t *q_start, *lens, *table;
     const int8_t *k, *v;
     const float *ks, *vs;
-    float scale_log2;  // scale * log2(e) * kCodeScale
+    float scale_log2;  // scale * log2(e)
     int window;        // INT_MAX: none
     int tile_cols, tiles;  // columns a workgroup takes, column tiles of a request
     int splits, chunk;     // workgroups that share a tile's keys, and how many keys each takes

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         }
         top = max_halves(top);
         const int e2 = range_shift(top);
-        to_score[c] = ldexpf(fabsf(a.scale_log2), -e2);  // (its sign goes to the queries)
+        to_score[c] = ldexpf(fabsf(a.scale_log2), kCodeShift - e2);  // (its sign goes to the queries)
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             f16x8 part[PARTS];

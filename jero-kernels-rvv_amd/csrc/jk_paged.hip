@@ -475,9 +475,10 @@ jk_status jk_paged_extend(jk_stream s, const jk_paged *p, const int32_t *n_new, 
         return fail(JK_TENSOR_BOUNDS, "paged_extend: %zu tokens exceed the int32 range", st->max_tokens);
     const StepDev sd{(int)st->max_tokens, st->q_start, st->slots, st->positions, st->requests, st->status};
     int32_t *lo = lens_out ? lens_out : p->lens, *fo = n_free_out ? n_free_out : p->n_free;
-    // one workgroup numbers up to this many tokens itself
-    if (st->max_tokens <= 2 * kPagedThreads) {
-        if (p->n_requests <= 256 && st->max_tokens <= 512)  // (few waves to a barrier)
+    // One workgroup numbers up to this many tokens itself: a second launch costs more until there are some ten a thread (16
+    // requests of 500 new tokens 10.8 us, 12.2 in two launches; 100 of 128 13.1 and 12.0).
+    if (st->max_tokens <= 8 * kPagedThreads) {
+        if (p->n_requests <= 256 && st->max_tokens <= 512)  // (few waves to a barrier: a step of 4 tokens 4.3 us on the GPU, 6.8 with 1024 threads)
             hipLaunchKernelGGL((paged_extend_kernel<true, 256>), dim3(1), dim3(256), 0, (hipStream_t)s, d, n_new, sd, lo,
                                fo);
         else
@@ -515,7 +516,9 @@ jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent
     if (col_blocks * groups > kMaxBlocks)
         return fail(JK_TENSOR_BOUNDS, "paged_reorder: a table of %zu x %zu is too large", p->n_requests, p->max_pages);
     const int w = (int)width;
-    if (groups * p->max_pages <= (size_t)4 * kPagedThreads) {
+    // (one cell a thread: 16 groups of 4 rows, 63 columns 20.6 us with the selection before it, 22.2 in two launches; of 8 rows, 126
+    // columns 27.6 and 24.1)
+    if (groups * p->max_pages <= (size_t)kPagedThreads) {
         if (width <= 8)
             hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 8>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d,
                                parent, w, status, lo, to);

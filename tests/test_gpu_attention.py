@@ -110,6 +110,24 @@ def test_long_context_split_over_workgroups(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 32)])
+def test_long_prompts_split_over_workgroups(gpu, dtype, hd, page):
+    """Chunks of prompts whose keys several workgroups share, beside a single token and a request of a few."""
+    check(gpu, case(gpu, dtype, [1500, 1100, 70], [263, 1, 9], page, 1, 8, hd, seed=3))
+    check(gpu, case(gpu, dtype, [2111], [257], page, 1, 8, hd, seed=4))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (96, 32)])
+def test_many_prompts(gpu, dtype, hd, page):
+    """So many columns that a workgroup takes the most of them, requests that end inside its tiles, and short ones."""
+    kv, grp = (4, 32) if dtype == "f32" else (8, 16)
+    lens = [65 + 9 * i for i in range(16)]
+    new = [65, 65, 1, 33] * 4
+    check(gpu, case(gpu, dtype, lens, new, page, kv, grp, hd, seed=5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_bounds_that_are_off_do_not_change_results(gpu, dtype):
     """max_len is a matter of speed: too small and too large a one give the same within rounding."""
     c = case(gpu, dtype, [900, 20], [1, 1], 32, 1, 4, 64, seed=5)
@@ -180,7 +198,7 @@ def test_queries_of_any_size(gpu):
     """Rows of very large and very small f32 queries keep their precision (each row is brought to f16's range)."""
     torch = gpu
     c = case(torch, "f32", [90, 70], [1, 20], 16, 1, 2, 64, seed=12)
-    for f in (1e-30, 1e-10, 1e10, 1e30):
+    for f in (1e-37, 1e-30, 1e-10, 1e10, 1e30):
         d = dict(c, q=c["q"] * f)
         check(torch, d, scale=64 ** -0.5 / f)
 

@@ -50,7 +50,7 @@ class Dev:
 
 
 @pytest.mark.parametrize("b,page,cap", [(1, 16, 1), (3, 16, 70), (64, 64, 2048), (5, 256, 3000), (1024, 32, 2500),
-                                        (1025, 16, 2048), (2500, 16, 6001)])
+                                        (1025, 16, 2048), (2500, 16, 6001), (7, 64, 8193), (2500, 16, 9000)])
 def test_extend_and_release(gpu, b, page, cap):
     rng = np.random.default_rng(b + page)
     max_pages = 12
@@ -92,7 +92,7 @@ def test_extend_out_of_place_leaves_the_old_state(gpu):
     assert first == [x.tolist() for x in d.out]
 
 
-@pytest.mark.parametrize("cap", [64, 5000])
+@pytest.mark.parametrize("cap", [64, 5000, 8200])
 def test_steps_that_do_not_fit_change_nothing(gpu, cap):
     d, ref = Dev(gpu, 3, 4, 5, 16, cap), R.Pages(3, 4, 5, 16)
     assert d.extend(ref, [20, 3, 0]) == 0
@@ -119,7 +119,7 @@ def test_no_tokens_at_all(gpu):
 
 
 @pytest.mark.parametrize("width,groups,page", [(1, 3, 16), (2, 5, 16), (4, 1, 32), (8, 3, 16), (9, 2, 16), (32, 2, 64),
-                                               (5, 205, 16)])
+                                               (5, 205, 16), (9, 120, 16)])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_reorder(gpu, width, groups, page, in_place):
     """A prompt in the first row of each group, then steps of a token a row, each after a reordering."""
