@@ -51,7 +51,7 @@ struct BeamDev {
     int groups, width, vocab, eos, segs;
     bool vec;
     key_t64 *keys;  // [rows][segs][width], largest first
-    float *stats;   // [rows][segs][2]: maximum, sum of exp(x - maximum)
+    float2 *stats;  // [rows][segs]: maximum, sum of exp(x - maximum)
 };
 
 // The segment's logits of one lane, in pieces of 16 bytes: element i of the lane is token base + tok(i).
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamDev a) {
             if (l == 0) a.keys[at * a.width + b] = last;
         }
     }
-    if (l == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = sum;
+    if (l == 0) a.stats[at] = make_float2(m, sum);
 }
 
 // One workgroup a group. A wave joins a row's segments: each lane holds the best untaken key of its segments
@@ -165,22 +165,35 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {
             if (l == 0) s_total[b][0] = a.scores[row], s_tok[b][0] = a.eos;
             continue;
         }
-        const float *st = a.stats + 2 * row * a.segs;
-        float m = -__builtin_inff();
-        for (int i = l; i < a.segs; i += 64) m = fmaxf(m, st[2 * i]);
-        m = wave_max64_dpp(m);
-        float sum = 0.0f;
-        for (int i = l; i < a.segs; i += 64)
-            if (st[2 * i] > -__builtin_inff()) sum += st[2 * i + 1] * __builtin_amdgcn_exp2f((st[2 * i] - m) * kLog2e);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        const float lse = logf(sum), score = a.scores[row];
+        const float score = a.scores[row];
         const key_t64 *keys = a.keys + row * a.segs * a.width;
-        if (a.segs * a.width <= kJoinKeys) {
-            for (int i = l; i < a.segs * a.width; i += 64) s_keys[w][i] = keys[i];
+        float2 st[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            st[i] = l + 64 * i < a.segs ? a.stats[row * a.segs + l + 64 * i] : make_float2(-__builtin_inff(), 0.0f);
+        // (the staging's loads go out together, and before the sums are looked at)
+        const int n_keys = a.segs * a.width;
+        if (n_keys <= kJoinKeys) {
+            key_t64 some[kJoinKeys / 64];
+#pragma unroll
+            for (int i = 0; i < kJoinKeys / 64; ++i)
+                if (64 * i < n_keys) some[i] = keys[min(l + 64 * i, n_keys - 1)];
+#pragma unroll
+            for (int i = 0; i < kJoinKeys / 64; ++i)
+                if (64 * i < n_keys) s_keys[w][l + 64 * i] = some[i];
             wave_lds_sync();
             keys = s_keys[w];
         }
+        float m = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) m = fmaxf(m, st[i].x);
+        m = wave_max64_dpp(m);
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (st[i].x > -__builtin_inff()) sum += st[i].y * __builtin_amdgcn_exp2f((st[i].x - m) * kLog2e);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        const float lse = logf(sum);
         key_t64 head[NS];
         int taken[NS];
 #pragma unroll
@@ -286,7 +299,7 @@ jk_status jk_beam_select(jk_stream s, const jk_beam_args *a, void *ws, size_t ws
                     ws, w.bytes);
     BeamDev d{a->logits, a->scores, a->done, a->scores_out, a->parents, a->tokens, a->done_out,
               a->stride ? a->stride : a->vocab, (int)a->groups, (int)a->width, (int)a->vocab, (int)a->eos, (int)w.segs,
-              false, static_cast<key_t64 *>(ws), reinterpret_cast<float *>(static_cast<char *>(ws) + w.keys)};
+              false, static_cast<key_t64 *>(ws), reinterpret_cast<float2 *>(static_cast<char *>(ws) + w.keys)};
     d.vec = (uintptr_t)a->logits % 16 == 0 && d.stride * es % 16 == 0;
     const size_t blocks = (w.rows * w.segs + 3) / 4;
     if (blocks >= (size_t)1 << 24) return fail(JK_TENSOR_BOUNDS, "beam_select: %zu rows of %zu logits are too many", w.rows, a->vocab);

@@ -263,79 +263,92 @@ __device__ __forceinline__ int parent_row(const int32_t *parent, int row, int wi
 template <int MW>
 __device__ __forceinline__ void reorder_column(const PagedDev &p, const int32_t *parent, int width, bool ok,
                                                const int32_t *lens, int32_t *table_out, int g, int j);
-template <bool TABLE, int MW>
-__global__ __launch_bounds__(kPagedThreads) void paged_reorder_plan_kernel(PagedDev p, const int32_t *parent, int width,
-                                                                           int32_t *status, int32_t *lens_out,
-                                                                           int32_t *table_out) {
-    __shared__ unsigned long long s_scan[17];
-    __shared__ long s_sum[17];
-    const int tid = threadIdx.x, mask = (1 << p.page_shift) - 1;
+template <bool TABLE, int MW, int TH>
+__global__ __launch_bounds__(TH) void paged_reorder_plan_kernel(PagedDev p, const int32_t *parent, int width, int32_t *status,
+                                                                int32_t *lens_out, int32_t *table_out) {
+    __shared__ int s_takes[2][TH / 64], s_flags[TH / 64];  // of a wave (passes in turn)
+    const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, mask = (1 << p.page_shift) - 1;
     const long cap = (long)p.max_pages << p.page_shift;
-    const int n_free = *p.n_free, per = kPagedThreads / width * width;
-    // needs(row): whether it takes a page; flags get what is wrong with its parent
-    auto look = [&](int row, int *len, long *flags) -> bool {
+    const int n_free = *p.n_free, per = TH / width * width;
+    // whether a row takes a page; flags get what is wrong with its parent
+    enum { kBadLength = 1, kNotOwned = 2 };
+    auto look = [&](int row, int *len, int *flags) -> bool {
         const int from = parent_row(parent, row, width);
         *len = p.lens[from];
         if (*len < 0 || *len > cap) {
-            *flags |= 1;
+            *flags |= kBadLength;
             return false;
         }
         if ((*len & mask) == 0) return false;
         const int j = *len >> p.page_shift;
         const int own = p.owned[(size_t)from * p.max_pages + j];
-        if (!page_ok(own, p.n_pages) || own != p.table[(size_t)from * p.max_pages + j]) *flags |= 1l << 32;
+        if (!page_ok(own, p.n_pages) || own != p.table[(size_t)from * p.max_pages + j]) *flags |= kNotOwned;
         return !page_ok(p.owned[(size_t)row * p.max_pages + j], p.n_pages);
     };
-    // sums: rows that take a page, threads that met a bad length (from bit 32) and a page not owned (from bit 48)
-    long found[1] = {0};
-    int len = 0;
-    bool takes = false;
     const bool one = p.n_requests <= per;  // (one pass: what it finds is kept)
-    for (int row = tid; row < p.n_requests; row += one ? p.n_requests : kPagedThreads) {
-        long f = 0;
-        takes = look(row, &len, &f);
-        found[0] = ((found[0] | ((f & 1) << 32) | ((f >> 32) << 48))) + takes;
+    int len = 0, flags = 0, need = 0;
+    unsigned long long takers = 0;
+    for (int r0 = 0; r0 < p.n_requests; r0 += per) {
+        const int row = r0 + tid;
+        takers = __ballot(tid < per && row < p.n_requests && look(row, &len, &flags));
+        need += __builtin_popcountll(takers);
     }
-    wg_sums(found, s_sum);
-    const long need = found[0] & 0xFFFFFFFFl;
-    const int st = ((found[0] >> 32) & 0xFFFF) || n_free < 0 || n_free > p.n_pages ? JK_PAGED_BAD_LENGTH
-                   : found[0] >> 48                                                ? JK_PAGED_NOT_OWNED
-                   : need > n_free                                                 ? JK_PAGED_NO_PAGES
-                                                                                   : JK_PAGED_OK;
-    __syncthreads();  // (every thread has read n_free)
+    const int met = (__ballot(flags & kBadLength) ? kBadLength : 0) | (__ballot(flags & kNotOwned) ? kNotOwned : 0);
+    if (l == 0) s_takes[0][w] = need, s_flags[w] = met;
+    __syncthreads();  // (every thread has read n_free and, where one pass is all, the lengths)
+    // pages that the waves before this one take, and all
+    auto waves = [&](int pass, int *all) {
+        int before = 0;
+        *all = 0;
+#pragma unroll
+        for (int i = 0; i < TH / 64; ++i) {
+            const int n = s_takes[pass & 1][i];
+            before += i < w ? n : 0;
+            *all += n;
+        }
+        return before;
+    };
+    int before = waves(0, &need), wrong = 0;
+#pragma unroll
+    for (int i = 0; i < TH / 64; ++i) wrong |= s_flags[i];
+    const int st = (wrong & kBadLength) || n_free < 0 || n_free > p.n_pages ? JK_PAGED_BAD_LENGTH
+                   : (wrong & kNotOwned)                                    ? JK_PAGED_NOT_OWNED
+                   : need > n_free                                          ? JK_PAGED_NO_PAGES
+                                                                            : JK_PAGED_OK;
     if (tid == 0) {
         *status = st;
-        if (st == JK_PAGED_OK) *p.n_free = n_free - (int)need;
+        if (st == JK_PAGED_OK) *p.n_free = n_free - need;
     }
     if (st != JK_PAGED_OK) {
         if (lens_out != p.lens)
-            for (int row = tid; row < p.n_requests; row += kPagedThreads) lens_out[row] = p.lens[row];
+            for (int row = tid; row < p.n_requests; row += TH) lens_out[row] = p.lens[row];
         if (TABLE && table_out != p.table)
-            for (int i = tid; i < p.n_requests * p.max_pages; i += kPagedThreads) table_out[i] = p.table[i];
+            for (int i = tid; i < p.n_requests * p.max_pages; i += TH) table_out[i] = p.table[i];
         return;
     }
-    int taken = 0;
-    for (int r0 = 0; r0 < p.n_requests; r0 += per) {
+    int taken = 0, pass = 1;
+    for (int r0 = 0; r0 < p.n_requests; r0 += per, ++pass) {
         const int row = r0 + tid;
         const bool live = tid < per && row < p.n_requests;
+        int sum = 0;
         if (!one) {
-            long f = 0;
-            takes = live && look(row, &len, &f);
+            takers = __ballot(live && look(row, &len, &flags));
+            if (l == 0) s_takes[pass & 1][w] = __builtin_popcountll(takers);
+            __syncthreads();  // (all have read the pass's lengths, and left the counts of the pass before the last)
+            before = waves(pass, &sum);
         }
-        takes = takes && live;
-        unsigned long long sum;
-        const int at = taken + (int)wg_scan((unsigned long long)takes, s_scan, &sum);  // (a barrier: all have read)
-        if (takes) {
+        if (takers >> l & 1) {
+            const int at = taken + before + __builtin_popcountll(takers & ((1ull << l) - 1));
             const int id = p.free_pages[n_free - 1 - at];
             p.owned[(size_t)row * p.max_pages + (len >> p.page_shift)] = page_ok(id, p.n_pages) ? id : -1;
         }
         if (live) lens_out[row] = len;
-        taken += (int)sum;
+        taken += sum;
     }
     if constexpr (TABLE) {
         __syncthreads();
         const int groups = p.n_requests / width;
-        for (int i = tid; i < groups * p.max_pages; i += kPagedThreads)
+        for (int i = tid; i < groups * p.max_pages; i += TH)
             reorder_column<MW>(p, parent, width, true, lens_out, table_out, i / p.max_pages, i % p.max_pages);
     }
 }
@@ -518,17 +531,22 @@ jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent
     const int w = (int)width;
     // (one cell a thread: 16 groups of 4 rows, 63 columns 20.6 us with the selection before it, 22.2 in two launches; of 8 rows, 126
     // columns 27.6 and 24.1)
-    if (groups * p->max_pages <= (size_t)kPagedThreads) {
-        if (width <= 8)
-            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 8>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d,
-                               parent, w, status, lo, to);
+    const size_t cells = groups * p->max_pages;
+    const hipStream_t hs = (hipStream_t)s;
+    if (cells <= (size_t)kPagedThreads) {
+        const bool few = cells <= 256 && p->n_requests <= 256 / width * width;
+        if (width <= 8 && few)
+            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 8, 256>), dim3(1), dim3(256), 0, hs, d, parent, w, status, lo, to);
+        else if (width <= 8)
+            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 8, kPagedThreads>), dim3(1), dim3(kPagedThreads), 0, hs, d, parent,
+                               w, status, lo, to);
         else
-            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 32>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d,
+            hipLaunchKernelGGL((paged_reorder_plan_kernel<true, 32, kPagedThreads>), dim3(1), dim3(kPagedThreads), 0, hs, d,
                                parent, w, status, lo, to);
         return check_launch("paged_reorder_plan_kernel");
     }
-    hipLaunchKernelGGL((paged_reorder_plan_kernel<false, 8>), dim3(1), dim3(kPagedThreads), 0, (hipStream_t)s, d, parent,
-                       w, status, lo, to);
+    hipLaunchKernelGGL((paged_reorder_plan_kernel<false, 8, kPagedThreads>), dim3(1), dim3(kPagedThreads), 0, hs, d, parent, w,
+                       status, lo, to);
     JK_TRY(check_launch("paged_reorder_plan_kernel"));
     const dim3 grid((unsigned)(col_blocks * groups));
     if (width <= 8)
