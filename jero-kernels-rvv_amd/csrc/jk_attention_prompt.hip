@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     const int pos_hi = w0 < cols ? rq.len - rq.count + (min(w0 + 32 * NC, cols) - 1) / a.grp : -1;
 
     f32x16 o[NC][DT];
-    float m[NC], lsum[NC], vref = 0.0f;
+    float m[NC], lsum[NC], vref = 0.0f, per = 0.0f;  // per: kWeight / vref, 0 while all values are
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         m[c] = kNegInf, lsum[c] = 0.0f;
@@ -207,7 +207,6 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             whole = whole && pages.head[i] >= 0;
         }
         const bool vmove = vtop > vref * kSlackV;
-        const float vref_new = vmove ? vtop : vref, per = vref_new > 0.0f ? kWeight / vref_new : 0.0f;
         if (!whole) {
             asm("" : "+v"(s[0][0].v[0]));  // (keeps the branch: few tiles need this, and selects would cost every tile)
 #pragma unroll
@@ -242,7 +241,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                 const float m_new = top > m[c] + kSlack ? top : m[c];
                 // (the first reference of a column comes from nothing: nothing is kept)
                 const float fade = m_new == m[c] ? 1.0f : exp2_fast(m[c] - m_new);
-                const float fade_o = vmove ? fade * (vref / vref_new) : fade;
+                const float fade_o = vmove ? fade * (vref / vtop) : fade;
                 m[c] = m_new;
                 lsum[c] *= fade;
 #pragma unroll
@@ -251,25 +250,30 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                     for (int e = 0; e < 16; ++e) o[c][t][e] *= fade_o;
             }
         }
-        vref = vref_new;
+        if (vmove) vref = vtop, per = kWeight / vtop;
 
         // 16 tokens at a time: their weights, and their share of the second product
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float vw = vs[i * PG / 4] * per;
             f16x8 wf[NC][PARTS];
+            // In f16 the factor vs / r of the weights goes into the exponent (a weight of nothing still counts 2^-60 there: its
+            // column's sum divides by it), in f32 an addend of both would round more than p may.
+            constexpr bool kInExponent = PARTS == 1;
+            const float vw = kInExponent ? fmaxf(vs[i * PG / 4] * per, kWeight * 0x1p-60f) : vs[i * PG / 4] * per;
+            const float shift = kInExponent ? __builtin_amdgcn_logf(vw) : 0.0f;
+            const float back = kInExponent ? __builtin_amdgcn_rcpf(vw) : 1.0f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const float m_use = m[c] == kNegInf ? 0.0f : m[c];
+                const float off = shift - (m[c] == kNegInf ? 0.0f : m[c]);
                 float y[8], sum[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     // (unseen: 2^-inf = 0)
-                    const float p = exp2_fast(__builtin_fmaf(s[i / 2][c].v[8 * (i % 2) + e], f[c][i * PG / 4], -m_use));
-                    sum[e % 2] += p;
-                    y[e] = p * vw;
+                    y[e] = exp2_fast(__builtin_fmaf(s[i / 2][c].v[8 * (i % 2) + e], f[c][i * PG / 4], off));
+                    sum[e % 2] += y[e];
+                    if (!kInExponent) y[e] *= vw;
                 }
-                lsum[c] += sum[0] + sum[1];
+                lsum[c] = __builtin_fmaf(sum[0] + sum[1], back, lsum[c]);
                 split_f16<PARTS>(y, wf[c]);
             }
 #pragma unroll
