@@ -13,6 +13,12 @@ namespace jk {
 // of its output the channels (HDP / 16) (4 g + i) + t. Of the keys it loads row n (16 bytes at a time), of the values
 // channels (HDP / 16) n + t of the eight tokens whose scores it holds, so that the loads of a wave cover whole rows
 // and nothing goes through LDS.
+// What bounds it: the cache's bytes, 2 a channel and token for all columns of the group, where requests are many (64 requests,
+// 290 thousand tokens, 8 kv heads of 128, bf16: 117 us, 5.2 TB/s, as fast as a copy); where one long request is cut
+// over the CUs, a tile's chain of loads, products and exponentials (32 thousand tokens 21 us, 3.2 TB/s, and 5 for the joining); and
+// with hundreds of columns the matrix units, of which a tile of 16 columns uses a quarter of what the prompt kernel's does. Waves
+// take tokens in turn and not columns because the few columns of a step are one tile, and its keys' loads need many
+// waves in flight: three a SIMD.
 // PARTS: f16 parts that f32 queries and probabilities are split into.
 template <typename T, int HDP, int PARTS>
 __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(AttnDev a) {
@@ -271,7 +277,8 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
 }
 
 // Joins the splits of one column a wave: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. The lanes first take a split each
-// (their factors), then four channels each, with G groups of lanes on every G-th split; four splits' loads in flight.
+// (their factors), then four channels each, with G groups of lanes on every G-th split; four splits' loads in flight. A second
+// launch's latency: 5 us for 32 rows of 33 splits (0.6 MB).
 template <typename T, int HDP>
 __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
     constexpr int LP = HDP / 4, G = 64 / LP;
@@ -352,7 +359,7 @@ static jk_status attn_check(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
 // 30 us; 512 after none 19 and 20 us, after 4000 105 and 70 us; 2048 after none 115 and 64 us.) A call that can hold both
 // launches both (the counts are known on the device only), except that the prompt kernel takes a lone request
 // whatever its length turns out to be.
-// The prompt kernel takes 256 columns a workgroup (one a CU, 159 us for the 4096-token prompt against 175 with 128) where
+// The prompt kernel takes 256 columns a workgroup (one a CU, 159 us for the 4096-token prompt, 175 with 128) where
 // there are two tiles a CU to level out their lengths, else 128 (two a CU: 64 us for 2048 tokens against 96).
 // Where there are fewer tiles than places, their keys are cut into chunks of one size for the whole call, a place's share of the work,
 // so that the last ones are not left with a long request or with a prompt's last tiles, which see the most keys. Up to kWholeLen

@@ -55,6 +55,9 @@ struct BeamDev {
 };
 
 // The segment's logits of one lane, in pieces of 16 bytes: element i of the lane is token base + tok(i).
+// What bounds it: the logits, read once and held in registers between the maximum, the sum and the selection. 128 rows of 128256 in
+// f32: 66 MB in 17.5 us, 3.8 TB/s; 4 rows of 32000 6.3 us, one wave's latency. Segments of 2048 give 63 waves a row, so that one
+// request's few rows already reach many CUs, and leave 32 logits a lane.
 template <typename T>
 __global__ __launch_bounds__(256) void beam_rows_kernel(BeamDev a) {
     typedef typename T::raw raw;
@@ -150,6 +153,8 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamDev a) {
 // first wave joins the group's rows in the same way, by their totals.
 // The keys are staged in LDS where a row has at most kJoinKeys of them (a vocabulary of 256k at a width of 8): a round's next key
 // then comes at LDS latency.
+// What bounds it: `width` rounds twice, each a maximum over the wave and the next key behind it; 16 groups of 8 rows of 63
+// segments 8 us, one of 4 rows 5.
 constexpr int kJoinWaves = 8, kJoinKeys = 1024;
 template <int NS>  // segments a lane holds (64 * NS at most)
 __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {

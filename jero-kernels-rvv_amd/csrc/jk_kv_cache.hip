@@ -46,7 +46,9 @@ __device__ __forceinline__ int run_length(const AppendArgs &a, int t0) {
 
 // Quantizes the runs of tokens of one page that begin among tokens [chunk * x, chunk * (x + 1)) for one head
 // of keys or values (blockIdx.y). One pass over the new values where the run's 8-element pieces fit kHeld a thread,
-// else a second one from the caches.
+// else a second one from the caches. What bounds it: the values read and the codes written once (a page's old codes twice
+// more where it is rescaled). 9360 tokens of prompts, f32, 8 heads of 128: 96 MB in 24 us, 3.9 TB/s of the 5.3 that a copy
+// reaches; a step of 48 requests 4.2 us, a launch and three rounds of loads.
 // A decode step has one-token runs in as many pages as requests, a prompt runs of whole pages, and the host does not know
 // which a call is. Up to 1024 tokens a workgroup takes one token by 64 threads (bf16, 8 heads of 128: a step of 1024 requests 58 us,
 // 132 by runs of a page; a prompt of 1024 tokens 16.7 and 17.5), beyond that a 512th of the tokens, up to a page, by 256 threads
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs a) {
 }
 
 // A thread turns the codes of 16 bytes of output (4 or 8) of one head and slot into values, four of them 256 apart with their
-// loads in flight together; blockIdx.y: keys, values.
+// loads in flight together; blockIdx.y: keys, values. 9360 slots, 8 heads of 128, to f32: 96 MB in 18 us, 5.3 TB/s.
 constexpr int kReadPieces = 4;
 struct ReadArgs {
     const int8_t *codes[2];
