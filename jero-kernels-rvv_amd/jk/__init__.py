@@ -833,6 +833,7 @@ class PagedC(C.Structure):
 
 
 class PagedStepC(C.Structure):
+    tensors = ()
     _fields_ = [("max_tokens", _sz), ("q_start", _vp), ("slots", _vp), ("positions", _vp), ("requests", _vp),
                 ("status", _vp)]
 
@@ -847,6 +848,7 @@ class AttnQ8ArgsC(C.Structure):
                 ("q_stride_token", _sz), ("q_stride_head", _sz), ("out_stride_token", _sz), ("out_stride_head", _sz),
                 ("n_requests", _sz), ("max_pages", _sz), ("q_start", _vp), ("lens", _vp), ("table", _vp),
                 ("max_new", _sz), ("max_len", _sz), ("scale", C.c_float), ("window", _sz)]
+    head_dim = None  # of the queries, where they are known (the C struct has the cache's)
 
 
 class BeamArgsC(C.Structure):
@@ -892,12 +894,20 @@ def _i32(*tensors):
             raise TensorBoundsError("a packed int32 tensor is needed")
 
 
+def _ints(n, *tensors):
+    """int32 tensors of n elements each (None: not given; an address is taken as it is)."""
+    for x in tensors:
+        if x is not None and type(x) is not int and (_code_of(x) != _I32 or x.numel() != n or not x.is_contiguous()):
+            raise TensorBoundsError(f"a packed int32 tensor of {n} elements is needed")
+
+
 def paged(lens, table, owned, free_pages, n_free, page: int) -> PagedC:
     """jk_paged of int32 device tensors: lens [requests], table and owned [requests][columns], free_pages
     [pages], n_free [1]."""
     _i32(lens, table, owned, free_pages, n_free)
     if table.shape != owned.shape or table.dim() != 2 or table.shape[0] != lens.numel():
         raise TensorBoundsError("table and owned need one row a request and the same columns")
+    _ints(1, n_free)
     return _held(PagedC(lens.numel(), table.shape[1], free_pages.numel(), page, _ptr(lens), _ptr(table), _ptr(owned),
                         _ptr(free_pages), _ptr(n_free)), lens, table, owned, free_pages, n_free)
 
@@ -907,6 +917,7 @@ def paged_step(q_start, slots, positions, requests, status) -> PagedStepC:
     _i32(q_start, slots, positions, requests, status)
     if not slots.numel() == positions.numel() == requests.numel():
         raise TensorBoundsError("slots, positions and requests need the same length")
+    _ints(1, status)
     return _held(PagedStepC(slots.numel(), _ptr(q_start), _ptr(slots), _ptr(positions), _ptr(requests), _ptr(status)),
                  q_start, slots, positions, requests, status)
 
@@ -918,17 +929,25 @@ def dev_paged_reset(p: PagedC, stream=None):
 
 def dev_paged_extend(p: PagedC, n_new, step: PagedStepC, lens_out=None, n_free_out=None, stream=None):
     """jk_paged_extend: n_new[r] more tokens for each request; pages, slots and positions of the step's tokens."""
+    _ints(p.n_requests, n_new, lens_out)
+    _ints(1, n_free_out)
+    if step.tensors and step.tensors[0].numel() != p.n_requests + 1:
+        raise TensorBoundsError("the step's q_start needs one element more than there are requests")
     _check(lib().jk_paged_extend(stream, C.byref(p), _ptr(n_new), C.byref(step), _ptr(lens_out),
                                  _ptr(n_free_out)))
 
 
 def dev_paged_release(p: PagedC, ended, stream=None):
     """jk_paged_release: the pages of the requests with ended[r] != 0 back on the stack."""
+    _ints(p.n_requests, ended)
     _check(lib().jk_paged_release(stream, C.byref(p), _ptr(ended)))
 
 
 def dev_paged_reorder(p: PagedC, parent, width: int, status, lens_out=None, table_out=None, stream=None):
     """jk_paged_reorder: row r of each group of `width` goes on from row parent[r]."""
+    _ints(p.n_requests, parent, lens_out)
+    _ints(1, status)
+    _ints(p.n_requests * p.max_pages, table_out)
     _check(lib().jk_paged_reorder(stream, C.byref(p), _ptr(parent), width, _ptr(status),
                                   _ptr(lens_out), _ptr(table_out)))
 
@@ -969,6 +988,8 @@ def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
 
 def dev_kv_reorder_q8(c: KvQ8C, p: PagedC, parent, width: int, status, stream=None):
     """jk_kv_reorder_q8: the cache's part of dev_paged_reorder, after it, for each layer."""
+    _ints(p.n_requests, parent)
+    _ints(1, status)
     _check(lib().jk_kv_reorder_q8(stream, C.byref(c), C.byref(p), _ptr(parent), width,
                                   _ptr(status)))
 
@@ -982,9 +1003,11 @@ def attn_q8_args(q, out, q_start, lens, table, max_new: int, max_len: int, scale
         raise TensorBoundsError("queries and output need the same shape and type")
     if table.dim() != 2 or table.shape[0] != lens.numel() or q_start.numel() != lens.numel() + 1:
         raise TensorBoundsError("one length and one row of the table a request and one more q_start are needed")
-    return _held(AttnQ8ArgsC(_ptr(q), _ptr(out), _dtype_of(q), q.shape[0], q.shape[1], qt, qh, ot, oh, lens.numel(),
+    args = _held(AttnQ8ArgsC(_ptr(q), _ptr(out), _dtype_of(q), q.shape[0], q.shape[1], qt, qh, ot, oh, lens.numel(),
                              table.shape[1], _ptr(q_start), _ptr(lens), _ptr(table), max_new, max_len, scale, window),
                  q, out, q_start, lens, table)
+    args.head_dim = q.shape[2]
+    return args
 
 
 def attn_q8_workspace_bytes(c: KvQ8C, a: AttnQ8ArgsC) -> int:
@@ -994,6 +1017,8 @@ def attn_q8_workspace_bytes(c: KvQ8C, a: AttnQ8ArgsC) -> int:
 
 def dev_attn_q8(c: KvQ8C, a: AttnQ8ArgsC, ws=None, stream=None, ws_bytes=None):
     """jk_attn_q8: causal attention of the step's queries over the paged 8-bit cache."""
+    if a.head_dim is not None and a.head_dim != c.head_dim:
+        raise TensorBoundsError(f"queries of {a.head_dim} channels for a cache of {c.head_dim}")
     _check(lib().jk_attn_q8(stream, C.byref(c), C.byref(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
 
 

@@ -90,3 +90,31 @@ def test_beam_and_page_arguments():
         jk.paged(ints(2), ints(3, 8), ints(3, 8), ints(9), ints(1), 16)
     with pytest.raises(TB):
         jk.paged_step(ints(3), ints(4), ints(5), ints(4), ints(1))
+
+
+def test_tables_and_flags_of_the_wrong_size_or_type():
+    """Counts, flags and parents are read one a request: the usual int64 tensor or a short one must not get that far."""
+    p = jk.paged(ints(6), ints(6, 8), ints(6, 8), ints(40), ints(1), 16)
+    step = jk.paged_step(ints(7), ints(9), ints(9), ints(9), ints(1))
+    calls = [lambda: jk.paged(ints(6), ints(6, 8), ints(6, 8), ints(40), ints(0), 16),
+             lambda: jk.paged_step(ints(7), ints(9), ints(9), ints(9), ints(2)),
+             lambda: jk.dev_paged_extend(p, ints(6), jk.paged_step(ints(6), ints(9), ints(9), ints(9), ints(1))),
+             lambda: jk.dev_paged_extend(p, ints(6), step, ints(5), ints(1)),
+             lambda: jk.dev_paged_extend(p, ints(6), step, ints(6), ints(1).long()),
+             lambda: jk.dev_paged_reorder(p, ints(2, 3), 3, ints(1).long()),
+             lambda: jk.dev_paged_reorder(p, ints(2, 3), 3, ints(1), ints(6), ints(6, 7)),
+             lambda: jk.dev_kv_reorder_q8(jk.kv_q8(*cache(40)), p, ints(2, 3), 3, ints(0))]
+    for x in (ints(5), ints(6).long(), ints(6, 2)[:, 0]):
+        calls += [lambda x=x: jk.dev_paged_extend(p, x, step), lambda x=x: jk.dev_paged_release(p, x),
+                  lambda x=x: jk.dev_paged_reorder(p, x, 3, ints(1)),
+                  lambda x=x: jk.dev_kv_reorder_q8(jk.kv_q8(*cache(40)), p, x, 3, ints(1))]
+    for call in calls:
+        with pytest.raises(TB):
+            call()
+
+
+def test_queries_of_another_head_dimension():
+    q = torch.zeros((5, 4, 80))
+    a = jk.attn_q8_args(q, torch.zeros_like(q), ints(3), ints(2), ints(2, 8), 1, 10, 0.125)
+    with pytest.raises(TB, match="80 channels"):
+        jk.dev_attn_q8(jk.kv_q8(*cache()), a)
