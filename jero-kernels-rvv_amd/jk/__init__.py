@@ -833,7 +833,7 @@ class PagedC(C.Structure):
 
 
 class PagedStepC(C.Structure):
-    tensors = ()
+    requests_held = None  # that q_start has room for, where that is known
     _fields_ = [("max_tokens", _sz), ("q_start", _vp), ("slots", _vp), ("positions", _vp), ("requests", _vp),
                 ("status", _vp)]
 
@@ -894,11 +894,14 @@ def _i32(*tensors):
             raise TensorBoundsError("a packed int32 tensor is needed")
 
 
-def _ints(n, *tensors):
-    """int32 tensors of n elements each (None: not given; an address is taken as it is)."""
-    for x in tensors:
-        if x is not None and type(x) is not int and (_code_of(x) != _I32 or x.numel() != n or not x.is_contiguous()):
-            raise TensorBoundsError(f"a packed int32 tensor of {n} elements is needed")
+def _ints(x, n: int) -> int:
+    """Address of a packed int32 tensor of n elements (0: not given; an address is taken as it is)."""
+    if x is None or type(x) is int:
+        return x or 0
+    # (these run in every step: the table first, its filling only for a type not met yet)
+    if (_dtype_codes.get(x.dtype) != _I32 and _code_of(x) != _I32) or x.numel() != n or not x.is_contiguous():
+        raise TensorBoundsError(f"a packed int32 tensor of {n} elements is needed")
+    return x.data_ptr()
 
 
 def paged(lens, table, owned, free_pages, n_free, page: int) -> PagedC:
@@ -907,7 +910,7 @@ def paged(lens, table, owned, free_pages, n_free, page: int) -> PagedC:
     _i32(lens, table, owned, free_pages, n_free)
     if table.shape != owned.shape or table.dim() != 2 or table.shape[0] != lens.numel():
         raise TensorBoundsError("table and owned need one row a request and the same columns")
-    _ints(1, n_free)
+    _ints(n_free, 1)
     return _held(PagedC(lens.numel(), table.shape[1], free_pages.numel(), page, _ptr(lens), _ptr(table), _ptr(owned),
                         _ptr(free_pages), _ptr(n_free)), lens, table, owned, free_pages, n_free)
 
@@ -917,39 +920,41 @@ def paged_step(q_start, slots, positions, requests, status) -> PagedStepC:
     _i32(q_start, slots, positions, requests, status)
     if not slots.numel() == positions.numel() == requests.numel():
         raise TensorBoundsError("slots, positions and requests need the same length")
-    _ints(1, status)
-    return _held(PagedStepC(slots.numel(), _ptr(q_start), _ptr(slots), _ptr(positions), _ptr(requests), _ptr(status)),
+    _ints(status, 1)
+    step = _held(PagedStepC(slots.numel(), _ptr(q_start), _ptr(slots), _ptr(positions), _ptr(requests), _ptr(status)),
                  q_start, slots, positions, requests, status)
+    step.requests_held = q_start.numel() - 1
+    return step
 
 
 def dev_paged_reset(p: PagedC, stream=None):
     """jk_paged_reset: empty requests, all pages free."""
-    _check(lib().jk_paged_reset(stream, C.byref(p)))
+    _check(lib().jk_paged_reset(stream, C.addressof(p)))
 
 
 def dev_paged_extend(p: PagedC, n_new, step: PagedStepC, lens_out=None, n_free_out=None, stream=None):
     """jk_paged_extend: n_new[r] more tokens for each request; pages, slots and positions of the step's tokens."""
-    _ints(p.n_requests, n_new, lens_out)
-    _ints(1, n_free_out)
-    if step.tensors and step.tensors[0].numel() != p.n_requests + 1:
+    n = p.n_requests
+    if step.requests_held not in (None, n):
         raise TensorBoundsError("the step's q_start needs one element more than there are requests")
-    _check(lib().jk_paged_extend(stream, C.byref(p), _ptr(n_new), C.byref(step), _ptr(lens_out),
-                                 _ptr(n_free_out)))
+    status = (_lib_handle or lib()).jk_paged_extend(stream, C.addressof(p), _ints(n_new, n), C.addressof(step),
+                                                    _ints(lens_out, n), _ints(n_free_out, 1))
+    if status:
+        _check(status)
 
 
 def dev_paged_release(p: PagedC, ended, stream=None):
     """jk_paged_release: the pages of the requests with ended[r] != 0 back on the stack."""
-    _ints(p.n_requests, ended)
-    _check(lib().jk_paged_release(stream, C.byref(p), _ptr(ended)))
+    _check(lib().jk_paged_release(stream, C.addressof(p), _ints(ended, p.n_requests)))
 
 
 def dev_paged_reorder(p: PagedC, parent, width: int, status, lens_out=None, table_out=None, stream=None):
     """jk_paged_reorder: row r of each group of `width` goes on from row parent[r]."""
-    _ints(p.n_requests, parent, lens_out)
-    _ints(1, status)
-    _ints(p.n_requests * p.max_pages, table_out)
-    _check(lib().jk_paged_reorder(stream, C.byref(p), _ptr(parent), width, _ptr(status),
-                                  _ptr(lens_out), _ptr(table_out)))
+    n = p.n_requests
+    failed = (_lib_handle or lib()).jk_paged_reorder(stream, C.addressof(p), _ints(parent, n), width, _ints(status, 1),
+                                                     _ints(lens_out, n), _ints(table_out, n * p.max_pages))
+    if failed:
+        _check(failed)
 
 
 def kv_q8(k, v, k_scale, v_scale) -> KvQ8C:
@@ -969,10 +974,9 @@ def dev_kv_append_q8(c: KvQ8C, k, v, slots, stream=None):
     n, kv, hd = k.shape
     if _strides(v) != (st, sh) or v.shape != k.shape or v.dtype != k.dtype:
         raise TensorBoundsError("keys and values need the same shape, strides and type")
-    if kv != c.n_kv or hd != c.head_dim or slots.numel() != n:
-        raise TensorBoundsError("keys of the cache's heads and one slot a token are needed")
-    _i32(slots)
-    _check(lib().jk_kv_append_q8(stream, C.byref(c), k.data_ptr(), v.data_ptr(), _dtype_of(k), n, st, sh, _ptr(slots)))
+    if kv != c.n_kv or hd != c.head_dim:
+        raise TensorBoundsError("keys of the cache's heads are needed")
+    _check(lib().jk_kv_append_q8(stream, C.addressof(c), k.data_ptr(), v.data_ptr(), _dtype_of(k), n, st, sh, _ints(slots, n)))
 
 
 def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
@@ -982,16 +986,14 @@ def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
     for x in outs:
         if not x.is_contiguous() or x.numel() != slots.numel() * c.n_kv * c.head_dim or x.dtype != outs[0].dtype:
             raise TensorBoundsError("outputs need packed tensors [slots][kv heads][head_dim] of one type")
-    _check(lib().jk_kv_read_q8(stream, C.byref(c), _ptr(slots), slots.numel(),
+    _check(lib().jk_kv_read_q8(stream, C.addressof(c), _ptr(slots), slots.numel(),
                                _dtype_of(outs[0]) if outs else F32, _ptr(k_out), _ptr(v_out)))
 
 
 def dev_kv_reorder_q8(c: KvQ8C, p: PagedC, parent, width: int, status, stream=None):
     """jk_kv_reorder_q8: the cache's part of dev_paged_reorder, after it, for each layer."""
-    _ints(p.n_requests, parent)
-    _ints(1, status)
-    _check(lib().jk_kv_reorder_q8(stream, C.byref(c), C.byref(p), _ptr(parent), width,
-                                  _ptr(status)))
+    _check(lib().jk_kv_reorder_q8(stream, C.addressof(c), C.addressof(p), _ints(parent, p.n_requests), width,
+                                  _ints(status, 1)))
 
 
 def attn_q8_args(q, out, q_start, lens, table, max_new: int, max_len: int, scale: float, window: int = 0) -> AttnQ8ArgsC:
@@ -1019,7 +1021,7 @@ def dev_attn_q8(c: KvQ8C, a: AttnQ8ArgsC, ws=None, stream=None, ws_bytes=None):
     """jk_attn_q8: causal attention of the step's queries over the paged 8-bit cache."""
     if a.head_dim is not None and a.head_dim != c.head_dim:
         raise TensorBoundsError(f"queries of {a.head_dim} channels for a cache of {c.head_dim}")
-    _check(lib().jk_attn_q8(stream, C.byref(c), C.byref(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
+    _check(lib().jk_attn_q8(stream, C.addressof(c), C.addressof(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
 
 
 def beam_args(logits, scores, done, scores_out, parents, tokens, done_out=None, eos: int = -1) -> BeamArgsC:
@@ -1049,7 +1051,7 @@ def beam_workspace_bytes(a: BeamArgsC) -> int:
 
 def dev_beam_select(a: BeamArgsC, ws, stream=None, ws_bytes=None):
     """jk_beam_select: the width best continuations of each group's hypotheses."""
-    _check(lib().jk_beam_select(stream, C.byref(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
+    _check(lib().jk_beam_select(stream, C.addressof(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
 
 
 def dev_measure_stream_read(buf, nbytes, sink, stream=None):
