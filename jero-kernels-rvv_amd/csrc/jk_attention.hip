@@ -15,7 +15,7 @@ namespace jk {
 // and nothing goes through LDS.
 // What bounds it: the cache's bytes, 2 a channel and token for all columns of the group, where requests are many (64 requests,
 // 290 thousand tokens, 8 kv heads of 128, bf16: 117 us, 5.2 TB/s, as fast as a copy); where one long request is cut
-// over the CUs, a tile's chain of loads, products and exponentials (32 thousand tokens 21 us, 3.2 TB/s, and 5 for the joining); and
+// over the CUs, a tile's chain of loads, products and exponentials (32 thousand tokens 21 us, 3.2 TB/s, and 4 for the joining); and
 // with hundreds of columns the matrix units, of which a tile of 16 columns uses a quarter of what the prompt kernel's does. Waves
 // take tokens in turn and not columns because the few columns of a step are one tile, and its keys' loads need many
 // waves in flight: three a SIMD.
@@ -278,22 +278,26 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
 
 // Joins the splits of one column a wave: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. The lanes first take a split each
 // (their factors), then four channels each, with G groups of lanes on every G-th split; four splits' loads in flight. A second
-// launch's latency: 5 us for 32 rows of 33 splits (0.6 MB).
-template <typename T, int HDP>
+// launch's latency: 4 us for 32 rows of 33 splits (0.6 MB).
+// WPR: waves that share a column's splits.
+template <typename T, int HDP, int WPR>
 __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
     constexpr int LP = HDP / 4, G = 64 / LP;
     __shared__ float s_f[4][kMaxSplits];
+    __shared__ float4 s_y[4][LP];
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long unit = (long)blockIdx.x * 4 + w;
+    const long unit = (long)blockIdx.x * (4 / WPR) + w / WPR;
     if (unit >= (long)a.n_tokens * a.n_heads) return;
     const int token = (int)(unit / a.n_heads), head = (int)(unit % a.n_heads), h = head / a.grp;
-    // the request of the token
-    if (token < a.q_start[0]) return;
-    int lo = 0, hi = a.n_requests;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid] <= token) lo = mid;
-        else hi = mid;
+    // the request of the token: the last of those that do not begin after it, 64 of them looked at together
+    int lo = 0;
+    for (int n = a.n_requests; n > 0;) {
+        const int step = (n + 63) / 64, probes = (n + step - 1) / step;
+        const unsigned long long before = __ballot(l < probes && a.q_start[lo + min(l * step, n - 1)] <= token);
+        if (!(before & 1)) return;
+        const int at = __builtin_popcountll(before) - 1;
+        lo += at * step;
+        n = step == 1 ? 0 : min(step, n - at * step);
     }
     const Req rq = request_of(a, lo);
     const int i = token - rq.first;
@@ -305,15 +309,23 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
     const Span sp = span_of(a, rq, c0, min(c0 + tile, cols));
     if (sp.active == 1) return;  // (written whole)
     const size_t at = (size_t)unit * a.pitch;
+    const float2 none = make_float2(kNegInf, 0.0f);
+    float2 ml[kMaxSplits / 64];
     float m = kNegInf, lsum = 0.0f;
-    for (int s = l; s < sp.active; s += 64) m = fmaxf(m, a.part_ml[at + s].x);
+#pragma unroll
+    for (int k = 0; k < kMaxSplits / 64; ++k) {
+        ml[k] = none;
+        if (64 * k < sp.active && l + 64 * k < sp.active) ml[k] = a.part_ml[at + l + 64 * k];
+        m = fmaxf(m, ml[k].x);
+    }
     m = wave_max64_dpp(m);
     const float m_use = m == kNegInf ? 0.0f : m;
-    for (int s = l; s < sp.active; s += 64) {
-        const float2 ml = a.part_ml[at + s];
-        const float f = exp2_fast(ml.x - m_use);
-        s_f[w][s] = f;
-        lsum += ml.x == kNegInf ? ml.y : ml.y * f;  // (0, or NaN)
+#pragma unroll
+    for (int k = 0; k < kMaxSplits / 64; ++k) {
+        if (64 * k >= sp.active) break;
+        const float f = exp2_fast(ml[k].x - m_use);
+        s_f[w][l + 64 * k] = f;
+        lsum += ml[k].x == kNegInf ? ml[k].y : ml[k].y * f;  // (0, or NaN)
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) lsum += __shfl_xor(lsum, o, 64);
@@ -322,7 +334,7 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
     float4 y = make_float4(0, 0, 0, 0);
     if (d < a.hd) {
 #pragma unroll 4
-        for (int s = l / LP; s < sp.active; s += G) {
+        for (int s = w % WPR * G + l / LP; s < sp.active; s += WPR * G) {
             const float4 o = *reinterpret_cast<const float4 *>(a.part_o + (at + s) * a.hd + d);
             const float f = s_f[w][s];
             y.x = fmaf(o.x, f, y.x), y.y = fmaf(o.y, f, y.y), y.z = fmaf(o.z, f, y.z), y.w = fmaf(o.w, f, y.w);
@@ -332,6 +344,16 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(AttnDev a) {
     for (int o = LP; o < 64; o <<= 1) {
         y.x += __shfl_xor(y.x, o, 64), y.y += __shfl_xor(y.y, o, 64);
         y.z += __shfl_xor(y.z, o, 64), y.w += __shfl_xor(y.w, o, 64);
+    }
+    if constexpr (WPR > 1) {  // (a workgroup is one column: its waves have all come here)
+        if (l < LP) s_y[w][l] = y;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int k = 1; k < WPR; ++k) {
+            const float4 z = s_y[k][l % LP];
+            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+        }
     }
     if (l < LP && d < a.hd) {
         const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
@@ -367,6 +389,9 @@ static jk_status attn_check(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
 // in two; one of 1000 12.4 and 14; of 2000 17.5 and 14. A prompt of 1024 tokens 34 us whole and 50 in two; two of 700 after 300
 // 39 and 75; 512 tokens after 500 33 and 38, but of 256 channels 64 and 56). Longer ones go down to kMinPromptChunk keys (512
 // tokens after 2000 52 us, with 1024 keys at least 64; 1024 after 1000 83 and 73).
+// Few rows are joined by four waves each, more by one (one step after 32 thousand tokens, 32 rows: 19.2 us with four, 20.1 with one; 8
+// after 16 thousand, 256 rows: 46.3 and 50.2; 31 after 8 thousand, 992 rows: 121.7 and 118.5; 2048 rows: 40.1 and 37.3).
+constexpr size_t kJoinByFour = 512;
 constexpr size_t kFewCols = 1024, kFewColsF32 = 2048, kMixedCols = 64, kMinChunk = 256, kMinPromptChunk = 512, kWholeLen = 1024;
 struct AttnPlan {
     size_t few_tiles, few_splits, few_chunk, many_cols, many_tiles, many_splits, many_chunk, few_cols, pitch;
@@ -403,6 +428,15 @@ static size_t attn_ws_bytes(const jk_kv_q8 *c, const jk_attn_q8_args *a, const A
     return p.pitch == 1 ? 0 : a->n_tokens * a->n_heads * p.pitch * (c->head_dim * 4 + 8);
 }
 
+template <typename T, int HDP>
+static void launch_join(hipStream_t s, const AttnDev &d) {
+    const size_t rows = (size_t)d.n_tokens * d.n_heads;
+    if (rows <= kJoinByFour)
+        hipLaunchKernelGGL((attn_q8_join_kernel<T, HDP, 4>), dim3((unsigned)rows), dim3(256), 0, s, d);
+    else
+        hipLaunchKernelGGL((attn_q8_join_kernel<T, HDP, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, d);
+}
+
 template <typename T, int PARTS>
 static jk_status launch_attn(hipStream_t s, int dtype, AttnDev d, const AttnPlan &p) {
     const size_t units = (size_t)d.n_requests * d.n_kv;
@@ -419,10 +453,9 @@ static jk_status launch_attn(hipStream_t s, int dtype, AttnDev d, const AttnPlan
         JK_TRY(launch_attn_prompt(s, dtype, d));
     }
     if (p.pitch == 1) return JK_OK;
-    const unsigned blocks = (unsigned)(((size_t)d.n_tokens * d.n_heads + 3) / 4);
-    if (d.hd <= 64) hipLaunchKernelGGL((attn_q8_join_kernel<T, 64>), dim3(blocks), dim3(256), 0, s, d);
-    else if (d.hd <= 128) hipLaunchKernelGGL((attn_q8_join_kernel<T, 128>), dim3(blocks), dim3(256), 0, s, d);
-    else hipLaunchKernelGGL((attn_q8_join_kernel<T, 256>), dim3(blocks), dim3(256), 0, s, d);
+    if (d.hd <= 64) launch_join<T, 64>(s, d);
+    else if (d.hd <= 128) launch_join<T, 128>(s, d);
+    else launch_join<T, 256>(s, d);
     return check_launch("attn_q8_join_kernel");
 }
 

@@ -110,6 +110,16 @@ def test_long_context_split_over_workgroups(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_split_rows_among_many_requests(gpu, dtype, hd):
+    """Long requests beside many short ones, some without new tokens: the joining finds each token's request."""
+    lens = [1 + i % 30 for i in range(100)] + [2700, 5, 2100]
+    new = [i % 3 // 2 for i in range(100)] + [2, 0, 1]
+    check(gpu, case(gpu, dtype, lens, new, 64, 1, 4, hd, seed=6))
+    check(gpu, case(gpu, dtype, lens[66:], new[66:], 16, 1, 20, hd, seed=7))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 32)])
 def test_long_prompts_split_over_workgroups(gpu, dtype, hd, page):
     """Chunks of prompts whose keys several workgroups share, beside a single token and a request of a few."""
