@@ -873,7 +873,10 @@ def _dtype_of(x) -> int:
 
 def _strides(x) -> tuple[int, int]:
     """Token and head strides of a [tokens][heads][head_dim] tensor whose last dimension is packed."""
-    shape, stride = x.shape, x.stride()
+    return _strides_of(x.shape, x.stride())
+
+
+def _strides_of(shape, stride) -> tuple[int, int]:
     if len(shape) != 3 or (shape[2] > 1 and stride[2] != 1):
         raise TensorBoundsError("a [tokens][heads][head_dim] tensor with a packed last dimension is needed")
     if (shape[0] > 1 and stride[0] == 0) or (shape[1] > 1 and stride[1] == 0):
@@ -970,24 +973,34 @@ def kv_q8(k, v, k_scale, v_scale) -> KvQ8C:
 
 def dev_kv_append_q8(c: KvQ8C, k, v, slots, stream=None):
     """jk_kv_append_q8: k and v [tokens][kv heads][head_dim] (the same strides) into their slots."""
-    st, sh = _strides(k)
-    n, kv, hd = k.shape
-    if _strides(v) != (st, sh) or v.shape != k.shape or v.dtype != k.dtype:
+    shape, stride = k.shape, k.stride()
+    st, sh = _strides_of(shape, stride)
+    if v.shape != shape or v.dtype != k.dtype or (v.stride() != stride and _strides(v) != (st, sh)):
         raise TensorBoundsError("keys and values need the same shape, strides and type")
+    n, kv, hd = shape
     if kv != c.n_kv or hd != c.head_dim:
         raise TensorBoundsError("keys of the cache's heads are needed")
-    _check(lib().jk_kv_append_q8(stream, C.addressof(c), k.data_ptr(), v.data_ptr(), _dtype_of(k), n, st, sh, _ints(slots, n)))
+    status = (_lib_handle or lib()).jk_kv_append_q8(stream, C.addressof(c), k.data_ptr(), v.data_ptr(), _dtype_of(k), n, st,
+                                                    sh, _ints(slots, n))
+    if status:
+        _check(status)
 
 
 def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
     """jk_kv_read_q8: the values of the slots, packed [slots][kv heads][head_dim]; either output may be None."""
-    _i32(slots)
-    outs = [x for x in (k_out, v_out) if x is not None]
-    for x in outs:
-        if not x.is_contiguous() or x.numel() != slots.numel() * c.n_kv * c.head_dim or x.dtype != outs[0].dtype:
-            raise TensorBoundsError("outputs need packed tensors [slots][kv heads][head_dim] of one type")
-    _check(lib().jk_kv_read_q8(stream, C.addressof(c), _ptr(slots), slots.numel(),
-                               _dtype_of(outs[0]) if outs else F32, _ptr(k_out), _ptr(v_out)))
+    n, dtype = slots.numel(), None
+    elements = n * c.n_kv * c.head_dim
+    for x in (k_out, v_out):
+        if x is not None:
+            if x.numel() != elements or not x.is_contiguous() or (dtype is not None and x.dtype != dtype):
+                raise TensorBoundsError("outputs need packed tensors [slots][kv heads][head_dim] of one type")
+            dtype, first = x.dtype, x
+    status = (_lib_handle or lib()).jk_kv_read_q8(stream, C.addressof(c), _ints(slots, n), n,
+                                                  F32 if dtype is None else _dtype_of(first),
+                                                  0 if k_out is None else k_out.data_ptr(),
+                                                  0 if v_out is None else v_out.data_ptr())
+    if status:
+        _check(status)
 
 
 def dev_kv_reorder_q8(c: KvQ8C, p: PagedC, parent, width: int, status, stream=None):
@@ -1021,7 +1034,9 @@ def dev_attn_q8(c: KvQ8C, a: AttnQ8ArgsC, ws=None, stream=None, ws_bytes=None):
     """jk_attn_q8: causal attention of the step's queries over the paged 8-bit cache."""
     if a.head_dim is not None and a.head_dim != c.head_dim:
         raise TensorBoundsError(f"queries of {a.head_dim} channels for a cache of {c.head_dim}")
-    _check(lib().jk_attn_q8(stream, C.addressof(c), C.addressof(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
+    status = (_lib_handle or lib()).jk_attn_q8(stream, C.addressof(c), C.addressof(a), _ptr(ws), _ws_bytes(ws, ws_bytes))
+    if status:
+        _check(status)
 
 
 def beam_args(logits, scores, done, scores_out, parents, tokens, done_out=None, eos: int = -1) -> BeamArgsC:
