@@ -1,6 +1,8 @@
 // jk_attention_prompt.hip -- attention over the paged 8-bit cache: the kernel for prompts.
 #include "jk_attention.hpp"
 
+#include <type_traits>
+
 namespace jk {
 
 // 32 NC NW columns of one request and kv head by NW waves of 32 NC columns each. 64 tokens at a time are widened to f16
@@ -9,7 +11,7 @@ namespace jk {
 //      8 channels of token lane % 32.
 //   V: [channel][64 tokens], the tokens of each 16 ordered 0-3, 8-11, 4-7, 12-15: a lane of the second product (rows =
 //      channels) reads the 8 tokens whose scores the first one left in that half of the wave.
-// A prompt of 4096 tokens, 32 query and 8 kv heads of 128, bf16: 158 us, 868 TFLOP/s of the products under the diagonal, where a
+// A prompt of 4096 tokens, 32 query and 8 kv heads of 128, bf16: 156 us, 880 TFLOP/s of the products under the diagonal, where a
 // large matrix product reaches 1185. What bounds it: each 32 x 32 x 16 instruction needs 1 KB from LDS, which gives 64 to 67
 // bytes a cycle to a CU however it is read; that is 4096 of the about 5000 cycles of a tile, and beside it run the matrix units
 // (2048) and the exponentials, sums and conversions (about 3200 on each SIMD). 64 columns a wave would halve the reads, but need all
@@ -101,30 +103,34 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         int head[PG];
         float ks[PG], vs[PG];
     };
-    auto fetch = [&](int t0, Pages &p) {
+    auto fetch = [&](int t0, Pages &p) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PG; ++i) p.head[i] = table[min(t0 + kSpan * i, t_last) >> a.page_shift];
     };
     const unsigned page_bytes = hd << a.page_shift;
     u32x4 kraw[KP];
     uint32_t vraw[VP][8];
-    auto load = [&](int t0, Pages &p) {
-        const int8_t *k[PG], *v[PG];
+    auto load = [&](int t0, Pages &p) __attribute__((always_inline)) {
+        size_t place[PG];  // of the tile's tokens in each page, keys and values alike
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
             p.head[i] = page_ok(p.head[i], a.n_pages) ? p.head[i] * a.n_kv + h : -1;
             const unsigned ph = max(p.head[i], 0);
             p.ks[i] = a.ks[ph];
             p.vs[i] = a.vs[ph];
-            const size_t at = (size_t)ph * page_bytes + (min(t0 + kSpan * i, t_last) & page_mask & ~(kSpan - 1)) * hd;
-            k[i] = a.k + at;
-            v[i] = a.v + at;
+            place[i] = (size_t)ph * page_bytes + (min(t0 + kSpan * i, t_last) & page_mask & ~(kSpan - 1)) * hd;
         }
         // (a wave's lanes stage tokens of one page, but for values where a page has 16 tokens in a tile or a row 64 channels)
-        auto pick = [&](const int8_t *const *base, int token) {
-            const int8_t *at = base[0];
+        auto pick = [&](int token) __attribute__((always_inline)) {
+            size_t at = place[0];
 #pragma unroll
-            for (int i = 1; i < PG; ++i) at = token >= kSpan * i ? base[i] : at;
+            for (int i = 1; i < PG; ++i) {
+                size_t other = place[i];
+                // (kept a value: a choice among an array's elements puts the array into scratch memory; 2048 tokens in pages of 16
+                // took 110 us so, and 91 now, in pages of 64 64)
+                asm("" : "+s"(other));
+                at = token >= kSpan * i ? other : at;
+            }
             return at;
         };
 #pragma unroll
@@ -132,21 +138,21 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             const int piece = tid + i * TH, t = piece / (HDP / 16), c = piece % (HDP / 16);
             if (w * 64 + i * TH >= KB) break;
             const unsigned off = (t % kSpan) * hd + (16u * c < hd ? 16u * c : 0u);
-            kraw[i] = *reinterpret_cast<const u32x4 *>(pick(k, (w * 64 + i * TH) / (HDP / 16)) + off);
+            kraw[i] = *reinterpret_cast<const u32x4 *>(a.k + pick((w * 64 + i * TH) / (HDP / 16)) + off);
         }
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
             const int block = tid + i * TH, tg = block / (HDP / 4), c = block % (HDP / 4) * 4;
             if (w * 64 + i * TH >= VB) break;
             const int t = 16 * (tg / 2) + 4 * (tg & 1);
-            const int8_t *at = pick(v, PG == 4 && HDP == 64 ? t : 16 * ((w * 64 + i * TH) / (HDP / 4) / 2));
+            const int8_t *at = a.v + pick(PG == 4 && HDP == 64 ? t : 16 * ((w * 64 + i * TH) / (HDP / 4) / 2));
             const unsigned off = (t % kSpan) * hd + ((unsigned)c < hd ? (unsigned)c : 0u);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 vraw[i][e] = *reinterpret_cast<const uint32_t *>(at + off + (e < 4 ? e : e + 4) * hd);
         }
     };
-    auto stage_k = [&](int buf) {
+    auto stage_k = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int piece = tid + i * TH, t = piece / (HDP / 16), c = piece % (HDP / 16);
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             *reinterpret_cast<f16x8 *>(&s_k[buf][t * kRowK + swz_k<HDP>(2 * c + 1, t)]) = hi;
         }
     };
-    auto stage_v = [&](int buf) {
+    auto stage_v = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
             const int block = tid + i * TH, tg = block / (HDP / 4), c = block % (HDP / 4) * 4;
@@ -176,7 +182,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     // The LDS reads of both products run kAhead matrix instructions ahead of their use (left alone, the compiler puts each read
     // right before its use and the wave waits out the LDS latency every time).
     constexpr int kAhead = PARTS == 2 ? 3 : 6;
-    auto scores = [&](int buf, Scores (&s)[2][NC]) {
+    auto scores = [&](int buf, Scores (&s)[2][NC]) __attribute__((always_inline)) {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -201,7 +207,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         }
         __builtin_amdgcn_sched_group_barrier(0x008, NC * PARTS * kAhead, 0);
     };
-    auto use = [&](int t0, int buf, const Pages &pages) {
+    auto use = [&](int t0, int buf, const Pages &pages) __attribute__((always_inline)) {
         Scores s[2][NC];
         scores(buf, s);
         float vs[PG], vtop = 0.0f;
@@ -312,8 +318,9 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         load(begin + 64, next);
         fetch(begin + 128, after);
         __syncthreads();
-        int buf = 0;
-        for (int t0 = begin; t0 < end; t0 += 64, buf ^= 1) {
+        // (two tiles a turn: each knows its half of LDS, which saves an addition a read, 2 us of the 158)
+        auto tile = [&](int t0, auto which) __attribute__((always_inline)) {
+            constexpr int buf = decltype(which)::value;
             // (a tile after, or wholly before the window of, all of the wave's columns is only staged)
             if (t0 <= pos_hi && (long)t0 + 63 > (long)pos_lo - a.window) use(t0, buf, now);
             stage_k(buf ^ 1);
@@ -322,6 +329,10 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             load(t0 + 128, next);
             fetch(t0 + 192, after);
             __syncthreads();
+        };
+        for (int t0 = begin; t0 < end; t0 += 128) {
+            tile(t0, std::integral_constant<int, 0>());
+            if (t0 + 64 < end) tile(t0 + 64, std::integral_constant<int, 1>());
         }
     }
 
