@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
             const float fade = m_new == m ? 1.0f : exp2_fast(m - m_new), fade_o = vmove ? fade * (vref / vref_new) : fade;
             m = m_new;
             vref = vref_new;
-            per = kWeight / vref;
+            per = vref > 0.0f ? kWeight / vref : 0.0f;
             lsum *= fade;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= fade_o;

@@ -1,0 +1,47 @@
+"""Attention where the scales of the cache's pages are far apart: zero, the smallest that are stored, and large ones in pages that
+a query does not see.
+
+The bound of an output is paged_ref.attention's: it is made of the values that the query sees, whatever the others are.
+"""
+import numpy as np
+import pytest
+
+import paged_ref as R
+import test_gpu_attention as A
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["f32", "f16", "bf16"]
+# (lengths, new tokens, kv heads, group): one token, drafts, chunks of few columns, and prompts past them
+SHAPES = {"step": ([200, 40, 90], [1, 1, 1], 2, 4), "draft": ([200, 70], [5, 3], 1, 4), "chunk": ([150, 96], [100, 60], 1, 3),
+          "prompt": ([290], [263], 1, 8)}
+
+
+def check(torch, c, window=0, **kw):
+    """As test_gpu_attention.check, with nothing allowed beside the bound but the spacing of the type's smallest numbers."""
+    got = A.run(torch, c, window, **kw)
+    want, bound = R.attention(c["q"].float().numpy(), *c["codes"], *c["scale"], c["q_start"], c["lens"], c["table"],
+                              c["hd"] ** -0.5, window, A.UNIT[c["dtype"]])
+    far = np.abs(got - want)
+    if c["dtype"] == "f16":  # (from 65520 on a result rounds to infinity: one that may lie there by its bound may be infinite)
+        far[((got == np.inf) & (want + bound >= 65520)) | ((got == -np.inf) & (want - bound <= -65520))] = 0
+    least = {"f32": 2.0 ** -145, "f16": 2.0 ** -24, "bf16": 2.0 ** -133}[c["dtype"]]
+    assert np.all(far <= bound + least), (float(np.nanmax(far / (bound + least))), bool(np.isnan(got).any()))
+
+
+def first_pages(c, n, value, what=1):
+    """The first n pages of every request (all: n = -1) at a scale of `value`."""
+    for row in c["table"]:
+        pages = row[row >= 0]
+        c["scale"][what][pages if n < 0 else pages[:n]] = value
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("page,n", [(64, 1), (16, 2), (32, 1), (16, 5), (64, -1)])
+def test_value_pages_of_zeros(gpu, dtype, shape, page, n):
+    """Warm-up, padding, a value head that is zero: alone, and with other pages behind them."""
+    lens, new, kv, grp = SHAPES[shape]
+    c = A.case(gpu, dtype, lens, new, page, kv, grp, 64, seed=page + n)
+    first_pages(c, n, 0.0)
+    check(gpu, c)
