@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
     f32x4 o[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f32x4{0, 0, 0, 0};
-    float m = kNegInf, lsum = 0.0f, vref = 0.0f, per = 0.0f;  // per: kWeight / vref, 0 while all values are
+    float m = kNegInf, lsum = 0.0f, vref = kLeastV, per = kWeight / kLeastV;  // per: kWeight / vref
 
     // Byte offsets of this lane's loads inside 16 tokens' rows. Channels past the head dimension are read
     // from the row's start: queries are 0 there, and outputs are not stored.
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
             const float fade = m_new == m ? 1.0f : exp2_fast(m - m_new), fade_o = vmove ? fade * (vref / vref_new) : fade;
             m = m_new;
             vref = vref_new;
-            per = vref > 0.0f ? kWeight / vref : 0.0f;
+            per = kWeight / vref;
             lsum *= fade;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= fade_o;

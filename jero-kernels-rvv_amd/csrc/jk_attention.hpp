@@ -33,6 +33,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // its maximum across lanes. Weights are p_j vs / r times kWeight: at most 16 * 2^8 * 8 = 2^15, which f16 holds, and what is
 // 2^-18 of the reference is still a normal number.
 constexpr float kSlack = 8.0f, kSlackV = 8.0f, kWeight = 16.0f;
+// The value scale that weights are taken against is at least this, so that kWeight / r is finite: the smallest scale that
+// the append stores is above 2^-126 and still gives weights of 2^-2 p.
+constexpr float kLeastV = 0x1p-120f;
 
 struct AttnDev {
     const void *q;

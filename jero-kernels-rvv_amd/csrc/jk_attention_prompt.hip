@@ -82,7 +82,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     const int pos_hi = w0 < cols ? rq.len - rq.count + (min(w0 + 32 * NC, cols) - 1) / a.grp : -1;
 
     f32x16 o[NC][DT];
-    float m[NC], lsum[NC], vref = 0.0f, per = 0.0f;  // per: kWeight / vref, 0 while all values are
+    float m[NC], lsum[NC], vref = kLeastV, per = kWeight / kLeastV;  // per: kWeight / vref
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         m[c] = kNegInf, lsum[c] = 0.0f;
@@ -342,8 +342,8 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         const float lall = sum_halves(lsum[c]);
         if (col >= cols) continue;
         const int token = rq.first + col / a.grp, head = h * a.grp + col % a.grp;
-        const float to_out = vref * (kCodeScale / kWeight);
-        const float inv = sp.active > 1 ? to_out : lall == 0.0f ? 0.0f : to_out / lall;
+        // (one after the other: their quotient can be too small for f32 where vref is)
+        const float to_out = vref * (kCodeScale / kWeight), inv = lall == 0.0f ? 0.0f : 1.0f / lall;
         const size_t at = ((size_t)token * a.n_heads + head) * a.pitch + split;
         typename T::raw *out = static_cast<typename T::raw *>(a.out) + (size_t)token * a.ot + (size_t)head * a.oh;
 #pragma unroll
@@ -354,11 +354,12 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                 if (d >= a.hd) continue;
                 if (sp.active > 1) {
                     *reinterpret_cast<float4 *>(a.part_o + at * a.hd + d) = make_float4(
-                        o[c][t][4 * e] * inv, o[c][t][4 * e + 1] * inv, o[c][t][4 * e + 2] * inv, o[c][t][4 * e + 3] * inv);
+                        o[c][t][4 * e] * to_out, o[c][t][4 * e + 1] * to_out, o[c][t][4 * e + 2] * to_out,
+                        o[c][t][4 * e + 3] * to_out);
                 } else {
                     typename T::raw y[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = T::down(o[c][t][4 * e + i] * inv);
+                    for (int i = 0; i < 4; ++i) y[i] = T::down(o[c][t][4 * e + i] * to_out * inv);
                     if (a.out_vec) __builtin_memcpy(__builtin_assume_aligned(out + d, 4 * sizeof(y[0])), y, sizeof y);
                     else
 #pragma unroll

@@ -45,3 +45,15 @@ def test_value_pages_of_zeros(gpu, dtype, shape, page, n):
     c = A.case(gpu, dtype, lens, new, page, kv, grp, 64, seed=page + n)
     first_pages(c, n, 0.0)
     check(gpu, c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("page,n", [(64, 1), (16, 4), (64, -1)])
+@pytest.mark.parametrize("largest", [2.0 ** -119, 2.0 ** -118, 2.0 ** -110])
+def test_the_smallest_values_that_are_stored(gpu, dtype, shape, page, n, largest):
+    """Pages whose largest value is just above what counts as zero: alone, and with ordinary pages behind them."""
+    lens, new, kv, grp = SHAPES[shape]
+    c = A.case(gpu, dtype, lens, new, page, kv, grp, 64, seed=page - n)
+    first_pages(c, n, np.float32(largest) / np.float32(127))
+    check(gpu, c)
