@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * u + i] = acc[i];
-            vs[u] = x.there[u] ? x.vs[u] : 0.0f;
+            vs[u] = x.vs[u];
         }
         if (!whole) {
             asm("" : "+v"(s[0]));  // (keeps the branch: few tiles need this, and selects would cost every tile)
@@ -165,6 +165,12 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
             for (int i = 0; i < 8; ++i) {
                 const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
                 if (!(x.there[i / 4] && t <= pos && pos - t < a.window)) s[i] = kNegInf;
+            }
+            // (a page that the column sees nothing of has no say in its reference: its scale may be of any size)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int t = t0 + 16 * u;
+                if (!(x.there[u] && t <= pos && pos - (t + 15) < a.window)) vs[u] = 0.0f;
             }
         }
         // scores are s * f, f one number a page and positive (0 becomes next to nothing: an unseen -inf stays one)
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
             top = fmaxf(top, fmaxf(fmaxf(s[4 * u], s[4 * u + 1]), fmaxf(s[4 * u + 2], s[4 * u + 3])) * f[u]);
         }
         const bool vmove = fmaxf(vs[0], vs[1]) > vref * kSlackV;
-        if (vmove || __any(top > m + kSlack)) {
+        if (__any(vmove || top > m + kSlack)) {
             top = max_rows(top);
             const float m_new = top > m + kSlack ? top : m, vref_new = vmove ? fmaxf(vs[0], vs[1]) : vref;
             // (the first reference of a column comes from nothing: nothing is kept)

@@ -8,8 +8,8 @@
 //   s_j = scale q.k_j,  p_j = exp(s_j - m),  l = sum p_j,  o = sum p_j v_j / l
 // with k_j = ks * codes and v_j = vs * codes, ks and vs one number per page and head. The products run on f16
 // matrix instructions: codes are exact in f16, ks multiplies the finished score, and vs joins the
-// probability: w_j = p_j vs / r with r the largest vs so far, so that w_j stays in f16's range whatever the values' size; o is
-// rescaled by r like by m. Scores are computed transposed (rows = tokens), so a lane that holds a column's
+// probability: w_j = p_j vs / r with r the largest vs so far of the pages that the column sees, so that w_j stays in f16's range
+// whatever the values' size, and no page that is hidden from a column costs its weights their bits; o is rescaled by r like by m. Scores are computed transposed (rows = tokens), so a lane that holds a column's
 // scores of four consecutive tokens holds them just as the second product's operand wants them: the order
 // of the tokens inside a matrix instruction is free as long as both of its operands agree on it.
 #pragma once

@@ -82,10 +82,10 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     const int pos_hi = w0 < cols ? rq.len - rq.count + (min(w0 + 32 * NC, cols) - 1) / a.grp : -1;
 
     f32x16 o[NC][DT];
-    float m[NC], lsum[NC], vref = kLeastV, per = kWeight / kLeastV;  // per: kWeight / vref
+    float m[NC], lsum[NC], vref[NC], per[NC];  // per: kWeight / vref
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        m[c] = kNegInf, lsum[c] = 0.0f;
+        m[c] = kNegInf, lsum[c] = 0.0f, vref[c] = kLeastV, per[c] = kWeight / kLeastV;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -210,15 +210,14 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     auto use = [&](int t0, int buf, const Pages &pages) __attribute__((always_inline)) {
         Scores s[2][NC];
         scores(buf, s);
-        float vs[PG], vtop = 0.0f;
+        float vs[NC][PG];
         bool whole = t0 + 63 <= pos_lo && pos_hi - t0 < a.window;
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
-            vs[i] = pages.head[i] >= 0 ? pages.vs[i] : 0.0f;
-            vtop = fmaxf(vtop, vs[i]);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) vs[c][i] = pages.vs[i];
             whole = whole && pages.head[i] >= 0;
         }
-        const bool vmove = vtop > vref * kSlackV;
         if (!whole) {
             asm("" : "+v"(s[0][0].v[0]));  // (keeps the branch: few tiles need this, and selects would cost every tile)
 #pragma unroll
@@ -233,14 +232,23 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                         x = behind >= 0 && behind < a.window ? x : kNegInf;
                     }
                 }
+            // (a page that a column sees nothing of has no say in its reference: its scale may be of any size)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < PG; ++i) {
+                    const int behind = pos[c] - (t0 + kSpan * i);
+                    vs[c][i] = pages.head[i] >= 0 && behind >= 0 && behind - (kSpan - 1) < a.window ? vs[c][i] : 0.0f;
+                }
         }
         // scores are s * f, f one number a group and positive (0 becomes next to nothing: an unseen -inf stays one)
         float f[NC][PG];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float top = kNegInf;
+            float top = kNegInf, vtop = 0.0f;
 #pragma unroll
             for (int i = 0; i < PG; ++i) {
+                vtop = fmaxf(vtop, vs[c][i]);
                 f[c][i] = pages.ks[i] * to_score[c];
                 f[c][i] = f[c][i] < 1e-37f ? 1e-37f : f[c][i];
                 float big = kNegInf;
@@ -248,13 +256,16 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                 for (int e = 0; e < 32 / PG; ++e) big = fmaxf(big, s[(32 / PG * i + e) / 16][c].v[(32 / PG * i + e) % 16]);
                 top = fmaxf(top, big * f[c][i]);
             }
-            if (vmove || __any(top > m[c] + kSlack)) {
+            const bool vmove = vtop > vref[c] * kSlackV;
+            if (__any(vmove || top > m[c] + kSlack)) {
                 top = max_halves(top);
                 const float m_new = top > m[c] + kSlack ? top : m[c];
                 // (the first reference of a column comes from nothing: nothing is kept)
                 const float fade = m_new == m[c] ? 1.0f : exp2_fast(m[c] - m_new);
-                const float fade_o = vmove ? fade * (vref / vtop) : fade;
+                const float fade_o = vmove ? fade * (vref[c] / vtop) : fade;
                 m[c] = m_new;
+                vref[c] = vmove ? vtop : vref[c];
+                per[c] = kWeight / vref[c];
                 lsum[c] *= fade;
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
@@ -262,7 +273,6 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                     for (int e = 0; e < 16; ++e) o[c][t][e] *= fade_o;
             }
         }
-        if (vmove) vref = vtop, per = kWeight / vtop;
 
         // 16 tokens at a time: their weights, and their share of the second product
 #pragma unroll
@@ -271,11 +281,11 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             // In f16 the factor vs / r of the weights goes into the exponent (a weight of nothing still counts 2^-60 there: its
             // column's sum divides by it), in f32 an addend of both would round more than p may.
             constexpr bool kInExponent = PARTS == 1;
-            const float vw = kInExponent ? fmaxf(vs[i * PG / 4] * per, kWeight * 0x1p-60f) : vs[i * PG / 4] * per;
-            const float shift = kInExponent ? __builtin_amdgcn_logf(vw) : 0.0f;
-            const float back = kInExponent ? __builtin_amdgcn_rcpf(vw) : 1.0f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
+                const float vs_per = vs[c][i * PG / 4] * per[c], vw = kInExponent ? fmaxf(vs_per, kWeight * 0x1p-60f) : vs_per;
+                const float shift = kInExponent ? __builtin_amdgcn_logf(vw) : 0.0f;
+                const float back = kInExponent ? __builtin_amdgcn_rcpf(vw) : 1.0f;
                 const float off = shift - (m[c] == kNegInf ? 0.0f : m[c]);
                 float y[8], sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -343,7 +353,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
         if (col >= cols) continue;
         const int token = rq.first + col / a.grp, head = h * a.grp + col % a.grp;
         // (one after the other: their quotient can be too small for f32 where vref is)
-        const float to_out = vref * (kCodeScale / kWeight), inv = lall == 0.0f ? 0.0f : 1.0f / lall;
+        const float to_out = vref[c] * (kCodeScale / kWeight), inv = lall == 0.0f ? 0.0f : 1.0f / lall;
         const size_t at = ((size_t)token * a.n_heads + head) * a.pitch + split;
         typename T::raw *out = static_cast<typename T::raw *>(a.out) + (size_t)token * a.ot + (size_t)head * a.oh;
 #pragma unroll

@@ -49,7 +49,7 @@ def test_value_pages_of_zeros(gpu, dtype, shape, page, n):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", list(SHAPES))
-@pytest.mark.parametrize("page,n", [(64, 1), (16, 4), (64, -1)])
+@pytest.mark.parametrize("page,n", [(64, 1), (16, 4), (16, 3), (64, -1)])
 @pytest.mark.parametrize("largest", [2.0 ** -119, 2.0 ** -118, 2.0 ** -110])
 def test_the_smallest_values_that_are_stored(gpu, dtype, shape, page, n, largest):
     """Pages whose largest value is just above what counts as zero: alone, and with ordinary pages behind them."""
@@ -57,3 +57,28 @@ def test_the_smallest_values_that_are_stored(gpu, dtype, shape, page, n, largest
     c = A.case(gpu, dtype, lens, new, page, kv, grp, 64, seed=page - n)
     first_pages(c, n, np.float32(largest) / np.float32(127))
     check(gpu, c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9])
+@pytest.mark.parametrize("new,grp", [(100, 3), (270, 8)])
+@pytest.mark.parametrize("held", [0, 5])
+def test_later_pages_of_large_values(gpu, dtype, page, ratio, new, grp, held):
+    """A prompt from its first token, and one behind a few: what a query does not see yet takes nothing from its result."""
+    c = A.case(gpu, dtype, [held + new], [new], page, 1, grp, 64, seed=page)
+    c["scale"][1][c["table"][0, 1]] *= ratio
+    c["scale"][1][c["table"][0, 3 if page == 16 else 0]] *= 1 if page == 64 else 30
+    check(gpu, c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("lens,new,grp,window", [([200, 130, 60], [1, 1, 1], 4, 9), ([200, 130], [20, 3], 4, 20), ([290], [263], 8, 17)])
+def test_pages_before_the_window(gpu, dtype, page, lens, new, grp, window):
+    """Large values that have left the window, beside small ones in it."""
+    c = A.case(gpu, dtype, lens, new, page, 1, grp, 64, seed=page + window)
+    for r, n in enumerate(lens):
+        c["scale"][1][c["table"][r, :(n - new[r] - window) // page]] *= 1e8
+        c["scale"][1][c["table"][r, 2]] *= 1e7
+    check(gpu, c, window=window)
