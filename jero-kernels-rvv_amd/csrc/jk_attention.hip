@@ -158,6 +158,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * u + i] = acc[i];
             vs[u] = x.vs[u];
+            f[u] = x.ks[u];
         }
         if (!whole) {
             asm("" : "+v"(s[0]));  // (keeps the branch: few tiles need this, and selects would cost every tile)
@@ -166,17 +167,18 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
                 const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
                 if (!(x.there[i / 4] && t <= pos && pos - t < a.window)) s[i] = kNegInf;
             }
-            // (a page that the column sees nothing of has no say in its reference: its scale may be of any size)
+            // (a page that the column sees nothing of has no say in its references: its scales, or those of what stands in
+            // for a missing page, may be of any size, or no numbers)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int t = t0 + 16 * u;
-                if (!(x.there[u] && t <= pos && pos - (t + 15) < a.window)) vs[u] = 0.0f;
+                if (!(x.there[u] && t <= pos && pos - (t + 15) < a.window)) vs[u] = f[u] = 0.0f;
             }
         }
         // scores are s * f, f one number a page and positive (0 becomes next to nothing: an unseen -inf stays one)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            f[u] = x.ks[u] * to_score;
+            f[u] *= to_score;
             f[u] = f[u] < 1e-37f ? 1e-37f : f[u];
             top = fmaxf(top, fmaxf(fmaxf(s[4 * u], s[4 * u + 1]), fmaxf(s[4 * u + 2], s[4 * u + 3])) * f[u]);
         }

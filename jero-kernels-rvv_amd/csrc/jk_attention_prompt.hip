@@ -210,12 +210,12 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     auto use = [&](int t0, int buf, const Pages &pages) __attribute__((always_inline)) {
         Scores s[2][NC];
         scores(buf, s);
-        float vs[NC][PG];
+        float vs[NC][PG], f[NC][PG];
         bool whole = t0 + 63 <= pos_lo && pos_hi - t0 < a.window;
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) vs[c][i] = pages.vs[i];
+            for (int c = 0; c < NC; ++c) vs[c][i] = pages.vs[i], f[c][i] = pages.ks[i] * to_score[c];
             whole = whole && pages.head[i] >= 0;
         }
         if (!whole) {
@@ -232,24 +232,25 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
                         x = behind >= 0 && behind < a.window ? x : kNegInf;
                     }
                 }
-            // (a page that a column sees nothing of has no say in its reference: its scale may be of any size)
+            // (a page that a column sees nothing of has no say in its references: its scales, or those of what stands in for a
+            // missing page, may be of any size, or no numbers)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int i = 0; i < PG; ++i) {
                     const int behind = pos[c] - (t0 + kSpan * i);
-                    vs[c][i] = pages.head[i] >= 0 && behind >= 0 && behind - (kSpan - 1) < a.window ? vs[c][i] : 0.0f;
+                    const bool seen = pages.head[i] >= 0 && behind >= 0 && behind - (kSpan - 1) < a.window;
+                    vs[c][i] = seen ? vs[c][i] : 0.0f;
+                    f[c][i] = seen ? f[c][i] : 0.0f;
                 }
         }
         // scores are s * f, f one number a group and positive (0 becomes next to nothing: an unseen -inf stays one)
-        float f[NC][PG];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float top = kNegInf, vtop = 0.0f;
 #pragma unroll
             for (int i = 0; i < PG; ++i) {
                 vtop = fmaxf(vtop, vs[c][i]);
-                f[c][i] = pages.ks[i] * to_score[c];
                 f[c][i] = f[c][i] < 1e-37f ? 1e-37f : f[c][i];
                 float big = kNegInf;
 #pragma unroll

@@ -82,3 +82,30 @@ def test_pages_before_the_window(gpu, dtype, page, lens, new, grp, window):
         c["scale"][1][c["table"][r, :(n - new[r] - window) // page]] *= 1e8
         c["scale"][1][c["table"][r, 2]] *= 1e7
     check(gpu, c, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("page", [16, 64])
+def test_missing_pages_beside_a_first_page_never_written(gpu, dtype, shape, page):
+    """Table entries that are no pages, in a cache whose page 0 holds whatever was there before: NaN scales."""
+    lens, new, kv, grp = SHAPES[shape]
+    for seed in range(100):
+        c = A.case(gpu, dtype, lens, new, page, kv, grp, 64, seed=seed, spare=6)
+        if not (c["table"] == 0).any():
+            break
+    assert np.isnan(c["scale"][0][0]).all() and np.isnan(c["scale"][1][0]).all()
+    c["table"][0, 1], c["table"][-1, 0] = -1, 2 ** 31 - 1
+    check(gpu, c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("lens,new,grp,window", [([200, 130, 60], [1, 1, 1], 4, 9), ([200, 130], [20, 3], 4, 20), ([390], [263], 8, 17)])
+def test_pages_that_no_query_sees_may_hold_anything(gpu, dtype, page, lens, new, grp, window):
+    """Pages that a sliding window has left behind for good, never written since."""
+    c = A.case(gpu, dtype, lens, new, page, 1, grp, 64, seed=page + window)
+    for r, n in enumerate(lens):
+        left = c["table"][r, :(n - new[r] - window + 1) // page]
+        c["scale"][0][left] = c["scale"][1][left] = np.nan
+    check(gpu, c, window=window)
