@@ -569,7 +569,8 @@ typedef struct jk_paged {
     size_t page;      /* tokens a page: 16, 32, 64, 128 or 256 */
     int32_t *lens;    /* [n_requests] tokens held */
     int32_t *table;   /* [n_requests][max_pages] page ids; -1 past the pages in use after a reset */
-    int32_t *owned;   /* [n_requests][max_pages] the page allocated for that place by that request, -1 for none.
+    int32_t *owned;   /* [n_requests][max_pages] the page allocated for that place by that request, -1 for none, -2 - page
+                       * for one that a reordering took the request back from and that it will begin again.
                        * The same array as table where requests share no pages (no jk_paged_reorder) */
     int32_t *free_pages; /* [n_pages] stack of the free page ids */
     int32_t *n_free;     /* [1] its height */
@@ -590,7 +591,8 @@ typedef enum jk_paged_status {
     JK_PAGED_NO_PAGES = 1,   /* fewer free pages than needed */
     JK_PAGED_TOO_LONG = 2,   /* a request would pass max_pages pages, or the step max_tokens tokens */
     JK_PAGED_BAD_LENGTH = 3, /* a negative length or count, a length past max_pages pages, n_free outside 0..n_pages */
-    JK_PAGED_NOT_OWNED = 4   /* jk_paged_reorder: the page that a parent is filling is not its own */
+    JK_PAGED_NOT_OWNED = 4,  /* jk_paged_reorder: the page that a parent is filling is not its own */
+    JK_PAGED_SHORTER = 5     /* jk_paged_reorder: a row would go back to fewer full pages than it holds */
 } jk_paged_status;
 
 /* Empty requests and all pages free: lens = 0, table = owned = -1, and a stack that gives page 0 first. */
@@ -612,8 +614,10 @@ jk_status jk_paged_release(jk_stream s, const jk_paged *p, const int32_t *ended)
  * is out of range). Full pages are shared: the row of the table becomes the parent's. The page that is still being
  * filled becomes a page of the row's own, owned[r][.], taken from the stack if it has none there; its
  * contents are moved by jk_kv_reorder_q8, once for each layer's cache. Columns past the pages in use
- * become -1. lens and table go to lens_out and table_out, or back into p where these are NULL (pass both
- * or neither); owned, the stack's height and status (as jk_paged_step) are in place. p->owned and
+ * become -1. A row's own full pages may be read by others, so no row can go back to fewer full pages than it
+ * holds (JK_PAGED_SHORTER, and nothing changes): the rows of a group are to be kept equally long, those of
+ * finished hypotheses among them. lens and table go to lens_out and table_out, or back into p where these
+ * are NULL (pass both or neither); owned, the stack's height and status (as jk_paged_step) are in place. p->owned and
  * p->table must be different arrays. */
 jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent, size_t width, int32_t *status,
                            int32_t *lens_out, int32_t *table_out);

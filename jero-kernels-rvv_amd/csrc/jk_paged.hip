@@ -20,6 +20,10 @@ struct PagedDev {
 
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return (int)(((long)tokens + (1 << shift) - 1) >> shift); }
 
+// The page that an entry of `owned` stands for, or -1. An id is a page of the row; -2 - id one that the row began and then went
+// back from, to the place's first token, by a reordering: nobody reads it, and the row begins it again when it comes back.
+__device__ __forceinline__ int owned_page(int v) { return v <= -2 ? -2 - v : v; }
+
 // Exclusive prefix sum over the workgroup of one value per thread (the low and high words of v
 // are summed apart: the callers' sums stay below 2^31). *total gets the sum. s: 17 words of LDS.
 __device__ __forceinline__ unsigned long long wg_scan(unsigned long long v, unsigned long long *s,
@@ -97,10 +101,15 @@ __global__ __launch_bounds__(TH) void paged_extend_kernel(PagedDev p, const int3
                                                                      int32_t *n_free_out) {
     __shared__ unsigned long long s_scan[17];
     __shared__ long s_sum[17 * 3];
-    __shared__ int s_tok[TH + 1], s_pg[TH + 1], s_len[TH];
+    __shared__ int s_tok[TH + 1], s_pg[TH + 1], s_len[TH], s_kept[TH];
     const int tid = threadIdx.x, page = 1 << p.page_shift;
     const long cap = (long)p.max_pages << p.page_shift;
     const int n_free = *p.n_free;
+    // the page that request r, about to begin its place j, has there already, or -1 (one array for both: there are none)
+    auto kept_at = [&](int r, int j) -> int {
+        const int v = p.owned == p.table ? -1 : p.owned[(size_t)r * p.max_pages + j];
+        return v <= -2 && page_ok(owned_page(v), p.n_pages) ? owned_page(v) : -1;
+    };
 
     // does the step fit? (totals in 64 bits: counts are not trusted yet)
     long tokens = 0, pages = 0, bad = (n_free < 0 || n_free > p.n_pages), over = 0;
@@ -112,7 +121,9 @@ __global__ __launch_bounds__(TH) void paged_extend_kernel(PagedDev p, const int3
         }
         if (len + n > cap) over = 1;
         tokens += n;
-        pages += ((len + n + page - 1) >> p.page_shift) - ((len + page - 1) >> p.page_shift);
+        const long held = (len + page - 1) >> p.page_shift, more = ((len + n + page - 1) >> p.page_shift) - held;
+        pages += more;
+        if (more && held < p.max_pages && kept_at(r, (int)held) >= 0) --pages;
     }
     long sums[3] = {tokens, pages, bad | (over << 32)};
     wg_sums(sums, s_sum);
@@ -141,13 +152,19 @@ __global__ __launch_bounds__(TH) void paged_extend_kernel(PagedDev p, const int3
     for (int r0 = 0; r0 < p.n_requests; r0 += TH) {
         const int r = r0 + tid, nr = min(TH, p.n_requests - r0);
         const int len = r < p.n_requests ? p.lens[r] : 0, n = r < p.n_requests ? n_new[r] : 0;
-        const int more = pages_of(len + n, p.page_shift) - pages_of(len, p.page_shift);
+        int more = pages_of(len + n, p.page_shift) - pages_of(len, p.page_shift), kept = -1;
+        if (more) kept = kept_at(r, pages_of(len, p.page_shift));
+        if (kept >= 0) {
+            --more;
+            p.table[(size_t)r * p.max_pages + pages_of(len, p.page_shift)] = kept;
+        }
         unsigned long long sum;
         const unsigned long long at = carry + wg_scan((unsigned long long)n | ((unsigned long long)more << 32),
                                                       s_scan, &sum);
         s_tok[tid] = (int)(uint32_t)at;
         s_pg[tid] = (int)(at >> 32);
         s_len[tid] = len;
+        s_kept[tid] = kept;
         if (r < p.n_requests) st.q_start[r] = (int)(uint32_t)at;
         carry += sum;
         if (tid == 0) {
@@ -159,17 +176,18 @@ __global__ __launch_bounds__(TH) void paged_extend_kernel(PagedDev p, const int3
         // new pages, one a thread: entry m is page m - s_pg of its request, from the top of the stack down
         for (int m = s_pg[0] + tid; m < s_pg[nr]; m += TH) {
             const int i = owner_of(s_pg, nr, m);
-            const int j = pages_of(s_len[i], p.page_shift) + m - s_pg[i];
+            const int j = pages_of(s_len[i], p.page_shift) + (s_kept[i] >= 0) + m - s_pg[i];
             const int id = p.free_pages[n_free - 1 - m];
             const size_t cell = (size_t)(r0 + i) * p.max_pages + j;
             p.table[cell] = p.owned[cell] = page_ok(id, p.n_pages) ? id : -1;
         }
         if constexpr (FILL) {
             for (int t = s_tok[0] + tid; t < s_tok[nr]; t += TH) {
-                const int i = owner_of(s_tok, nr, t), held = pages_of(s_len[i], p.page_shift);
+                const int i = owner_of(s_tok, nr, t), held = pages_of(s_len[i], p.page_shift), kept = s_kept[i];
                 const int pos = s_len[i] + t - s_tok[i], j = pos >> p.page_shift;
-                const int id = j < held ? p.table[(size_t)(r0 + i) * p.max_pages + j]
-                                        : p.free_pages[n_free - 1 - (s_pg[i] + j - held)];
+                const int id = j < held                ? p.table[(size_t)(r0 + i) * p.max_pages + j]
+                               : kept >= 0 && j == held ? kept
+                                                        : p.free_pages[n_free - 1 - (s_pg[i] + j - held - (kept >= 0))];
                 write_token(st, t, page_ok(id, p.n_pages) ? (id << p.page_shift) + (pos & (page - 1)) : -1, pos,
                             r0 + i);
             }
@@ -224,7 +242,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p
             int n = 0;
             if (ended[r0 + i])
                 for (int j = l; j < p.max_pages; j += 64)
-                    n += page_ok(p.owned[(size_t)(r0 + i) * p.max_pages + j], p.n_pages);
+                    n += page_ok(owned_page(p.owned[(size_t)(r0 + i) * p.max_pages + j]), p.n_pages);
             n = wave_sum64_dpp(n);
             if (l == 0) s_cnt[i] = n;
         }
@@ -241,7 +259,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p
             for (int j0 = 0; j0 < p.max_pages; j0 += 64) {
                 const int j = j0 + l;
                 const size_t cell = (size_t)(r0 + i) * p.max_pages + j;
-                const int id = j < p.max_pages ? p.owned[cell] : -1;
+                const int id = j < p.max_pages ? owned_page(p.owned[cell]) : -1;
                 const unsigned long long has = __ballot(page_ok(id, p.n_pages));
                 const long to = at + __popcll(has & ((1ull << l) - 1));
                 if (page_ok(id, p.n_pages) && to < p.n_pages) p.free_pages[to] = id;
@@ -280,29 +298,37 @@ __global__ __launch_bounds__(TH) void paged_reorder_plan_kernel(PagedDev p, cons
     const long cap = (long)p.max_pages << p.page_shift;
     const int n_free = *p.n_free, per = TH / width * width;
     // whether a row takes a page; flags get what is wrong with its parent
-    enum { kBadLength = 1, kNotOwned = 2 };
-    auto look = [&](int row, int *len, int *flags) -> bool {
-        const int from = parent_row(parent, row, width);
-        *len = p.lens[from];
-        if (*len < 0 || *len > cap) {
+    enum { kBadLength = 1, kNotOwned = 2, kShorter = 4 };
+    struct Row {
+        int len, old, mine;  // its new length, the one that it had, and what `owned` has for it at the open page's place
+    };
+    auto look = [&](int row, Row *x, int *flags) -> bool {
+        const int from = parent_row(parent, row, width), len = p.lens[from], old = p.lens[row];
+        *x = Row{len, old, -1};
+        if (len < 0 || len > cap || old < 0 || old > cap) {
             *flags |= kBadLength;
             return false;
         }
-        if ((*len & mask) == 0) return false;
-        const int j = *len >> p.page_shift;
-        const int own = p.owned[(size_t)from * p.max_pages + j];
+        // (a row's full pages may be read by others: it must not come back to fill one of them again)
+        const int j = len >> p.page_shift;
+        if (j < old >> p.page_shift) *flags |= kShorter;
+        if ((len & mask) == 0) return false;
+        const int own = owned_page(p.owned[(size_t)from * p.max_pages + j]);
         if (!page_ok(own, p.n_pages) || own != p.table[(size_t)from * p.max_pages + j]) *flags |= kNotOwned;
-        return !page_ok(p.owned[(size_t)row * p.max_pages + j], p.n_pages);
+        x->mine = p.owned[(size_t)row * p.max_pages + j];
+        return !page_ok(owned_page(x->mine), p.n_pages);
     };
     const bool one = p.n_requests <= per;  // (one pass: what it finds is kept)
-    int len = 0, flags = 0, need = 0;
+    Row x{};
+    int flags = 0, need = 0;
     unsigned long long takers = 0;
     for (int r0 = 0; r0 < p.n_requests; r0 += per) {
         const int row = r0 + tid;
-        takers = __ballot(tid < per && row < p.n_requests && look(row, &len, &flags));
+        takers = __ballot(tid < per && row < p.n_requests && look(row, &x, &flags));
         need += __builtin_popcountll(takers);
     }
-    const int met = (__ballot(flags & kBadLength) ? kBadLength : 0) | (__ballot(flags & kNotOwned) ? kNotOwned : 0);
+    const int met = (__ballot(flags & kBadLength) ? kBadLength : 0) | (__ballot(flags & kNotOwned) ? kNotOwned : 0) |
+                    (__ballot(flags & kShorter) ? kShorter : 0);
     if (l == 0) s_takes[0][w] = need, s_flags[w] = met;
     __syncthreads();  // (every thread has read n_free and, where one pass is all, the lengths)
     // pages that the waves before this one take, and all
@@ -322,6 +348,7 @@ __global__ __launch_bounds__(TH) void paged_reorder_plan_kernel(PagedDev p, cons
     for (int i = 0; i < TH / 64; ++i) wrong |= s_flags[i];
     const int st = (wrong & kBadLength) || n_free < 0 || n_free > p.n_pages ? JK_PAGED_BAD_LENGTH
                    : (wrong & kNotOwned)                                    ? JK_PAGED_NOT_OWNED
+                   : (wrong & kShorter)                                     ? JK_PAGED_SHORTER
                    : need > n_free                                          ? JK_PAGED_NO_PAGES
                                                                             : JK_PAGED_OK;
     if (tid == 0) {
@@ -341,17 +368,24 @@ __global__ __launch_bounds__(TH) void paged_reorder_plan_kernel(PagedDev p, cons
         const bool live = tid < per && row < p.n_requests;
         int sum = 0;
         if (!one) {
-            takers = __ballot(live && look(row, &len, &flags));
+            takers = __ballot(live && look(row, &x, &flags));
             if (l == 0) s_takes[pass & 1][w] = __builtin_popcountll(takers);
             __syncthreads();  // (all have read the pass's lengths, and left the counts of the pass before the last)
             before = waves(pass, &sum);
         }
-        if (takers >> l & 1) {
-            const int at = taken + before + __builtin_popcountll(takers & ((1ull << l) - 1));
-            const int id = p.free_pages[n_free - 1 - at];
-            p.owned[(size_t)row * p.max_pages + (len >> p.page_shift)] = page_ok(id, p.n_pages) ? id : -1;
+        if (live) {
+            const int held = pages_of(x.len, p.page_shift);
+            int32_t *cells = p.owned + (size_t)row * p.max_pages;
+            if (takers >> l & 1) {
+                const int at = taken + before + __builtin_popcountll(takers & ((1ull << l) - 1));
+                const int id = p.free_pages[n_free - 1 - at];
+                cells[held - 1] = page_ok(id, p.n_pages) ? id : -1;
+            } else if (x.mine <= -2) {  // come back to the page that it went back from
+                cells[held - 1] = owned_page(x.mine);
+            }
+            if (held < pages_of(x.old, p.page_shift) && cells[held] >= 0) cells[held] = -2 - cells[held];  // goes back from it
+            lens_out[row] = x.len;
         }
-        if (live) lens_out[row] = len;
         taken += sum;
     }
     if constexpr (TABLE) {
@@ -419,7 +453,8 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(PagedDev p, jk_kv_q8 c,
         const int row = row0 + b, from = parent_row(parent, row, width), len = p.lens[row];
         if (from == row || len <= 0 || len > cap || (len & mask) == 0) continue;
         const int j = len >> p.page_shift;
-        const int src = p.owned[(size_t)from * p.max_pages + j], dst = p.owned[(size_t)row * p.max_pages + j];
+        const int src = owned_page(p.owned[(size_t)from * p.max_pages + j]);
+        const int dst = p.owned[(size_t)row * p.max_pages + j];
         if (!page_ok(src, p.n_pages) || !page_ok(dst, p.n_pages) || i * 16 >= (len & mask) * hd) continue;
         moves[b] = true;
         const size_t from_head = (size_t)src * heads + h;

@@ -821,7 +821,7 @@ def op_counts() -> tuple[int, int]:
 
 # ------------------------------------------- paged 8-bit attention cache, beam search
 F32, F16, BF16 = 0, 1, 30  # jk_dtype
-PAGED_OK, PAGED_NO_PAGES, PAGED_TOO_LONG, PAGED_BAD_LENGTH, PAGED_NOT_OWNED = 0, 1, 2, 3, 4
+PAGED_OK, PAGED_NO_PAGES, PAGED_TOO_LONG, PAGED_BAD_LENGTH, PAGED_NOT_OWNED, PAGED_SHORTER = 0, 1, 2, 3, 4, 5
 _I32 = -1  # (of the index arrays; not a jk_dtype)
 _DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int32": _I32}
 _dtype_codes = {}  # the same by dtype object, filled as they are met (a name costs more than a call's other checks)
