@@ -570,7 +570,8 @@ typedef struct jk_paged {
     int32_t *lens;    /* [n_requests] tokens held */
     int32_t *table;   /* [n_requests][max_pages] page ids; -1 past the pages in use after a reset */
     int32_t *owned;   /* [n_requests][max_pages] the page allocated for that place by that request, -1 for none, -2 - page
-                       * for one that a reordering took the request back from and that it will begin again.
+                       * for one that a reordering took the request back from and that it will begin again. Ids past the
+                       * pages in use (of a step that was dropped) do not count: those pages are on the stack.
                        * The same array as table where requests share no pages (no jk_paged_reorder) */
     int32_t *free_pages; /* [n_pages] stack of the free page ids */
     int32_t *n_free;     /* [1] its height */
@@ -600,12 +601,14 @@ jk_status jk_paged_reset(jk_stream s, const jk_paged *p);
 /* Adds n_new[r] tokens (device, 0 or more) to each request r. Pages that begin in the step are taken
  * from the top of the stack, request by request. The new lengths and stack height go to lens_out
  * [n_requests] and n_free_out [1], or back into p where these are NULL; a caller that passes its own
- * can drop the step (drafted tokens that were refused) by going on from the old ones. The stack itself is only
- * read. If the step does not fit, status says why and nothing else changes but the step's outputs:
+ * can drop the step (drafted tokens that were refused) by going on from the old ones, before any other
+ * call for these pages. What the step wrote past the old lengths in table and owned then no longer counts;
+ * of its tokens those that are taken up again are appended again, since their slots may be others. The
+ * stack itself is only read. If the step does not fit, status says why and nothing else changes but the step's outputs:
  * q_start is 0, slots, positions and requests are -1, and lens_out and n_free_out are copies. */
 jk_status jk_paged_extend(jk_stream s, const jk_paged *p, const int32_t *n_new, const jk_paged_step *step,
                           int32_t *lens_out, int32_t *n_free_out);
-/* Ends the requests r with ended[r] != 0 (device, [n_requests]): their owned pages go back on the stack in
+/* Ends the requests r with ended[r] != 0 (device, [n_requests]): the pages that they own go back on the stack in
  * order of request and place, their rows to -1 and their lengths to 0. Requests that share pages
  * (after jk_paged_reorder) are to be ended together. */
 jk_status jk_paged_release(jk_stream s, const jk_paged *p, const int32_t *ended);
@@ -617,8 +620,8 @@ jk_status jk_paged_release(jk_stream s, const jk_paged *p, const int32_t *ended)
  * become -1. A row's own full pages may be read by others, so no row can go back to fewer full pages than it
  * holds (JK_PAGED_SHORTER, and nothing changes): the rows of a group are to be kept equally long, those of
  * finished hypotheses among them. lens and table go to lens_out and table_out, or back into p where these
- * are NULL (pass both or neither); owned, the stack's height and status (as jk_paged_step) are in place. p->owned and
- * p->table must be different arrays. */
+ * are NULL (pass both or neither); owned, the stack's height and status (as jk_paged_step) are in place, so a
+ * reordering is not to be dropped. p->owned and p->table must be different arrays. */
 jk_status jk_paged_reorder(jk_stream s, const jk_paged *p, const int32_t *parent, size_t width, int32_t *status,
                            int32_t *lens_out, int32_t *table_out);
 

@@ -20,9 +20,11 @@ struct PagedDev {
 
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return (int)(((long)tokens + (1 << shift) - 1) >> shift); }
 
-// The page that an entry of `owned` stands for, or -1. An id is a page of the row; -2 - id one that the row began and then went
-// back from, to the place's first token, by a reordering: nobody reads it, and the row begins it again when it comes back.
-__device__ __forceinline__ int owned_page(int v) { return v <= -2 ? -2 - v : v; }
+// The page that an entry of `owned` stands for, or -1. An id is a page of the row where its place lies below the pages that the
+// row's tokens reach (`used`); past them it is left of a step that was dropped, and that page is on the stack or somebody else's.
+// -2 - id is a page that the row began and then went back from, to the place's first token, by a reordering: nobody reads it, and
+// the row begins it again when it comes back.
+__device__ __forceinline__ int owned_page(int v, bool used) { return v <= -2 ? -2 - v : used ? v : -1; }
 
 // Exclusive prefix sum over the workgroup of one value per thread (the low and high words of v
 // are summed apart: the callers' sums stay below 2^31). *total gets the sum. s: 17 words of LDS.
@@ -108,7 +110,7 @@ __global__ __launch_bounds__(TH) void paged_extend_kernel(PagedDev p, const int3
     // the page that request r, about to begin its place j, has there already, or -1 (one array for both: there are none)
     auto kept_at = [&](int r, int j) -> int {
         const int v = p.owned == p.table ? -1 : p.owned[(size_t)r * p.max_pages + j];
-        return v <= -2 && page_ok(owned_page(v), p.n_pages) ? owned_page(v) : -1;
+        return page_ok(owned_page(v, false), p.n_pages) ? owned_page(v, false) : -1;
     };
 
     // does the step fit? (totals in 64 bits: counts are not trusted yet)
@@ -236,13 +238,20 @@ __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p
     __shared__ int s_cnt[kPagedThreads];
     const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
     long height = min(max(*p.n_free, 0), p.n_pages);
+    auto pages_held = [&](int r) { return min(pages_of(max(p.lens[r], 0), p.page_shift), p.max_pages); };
+    // the page that request r owns at place j < max_pages, of `held` in use (one array for both: none is marked)
+    auto own = [&](int r, int j, int held) {
+        const int v = p.owned[(size_t)r * p.max_pages + j];
+        return p.owned == p.table && v < 0 ? -1 : owned_page(v, j < held);
+    };
     for (int r0 = 0; r0 < p.n_requests; r0 += kPagedThreads) {
         const int nr = min(kPagedThreads, p.n_requests - r0);
         for (int i = w; i < nr; i += kPagedThreads / 64) {
             int n = 0;
-            if (ended[r0 + i])
-                for (int j = l; j < p.max_pages; j += 64)
-                    n += page_ok(owned_page(p.owned[(size_t)(r0 + i) * p.max_pages + j]), p.n_pages);
+            if (ended[r0 + i]) {
+                const int held = pages_held(r0 + i);
+                for (int j = l; j < p.max_pages; j += 64) n += page_ok(own(r0 + i, j, held), p.n_pages);
+            }
             n = wave_sum64_dpp(n);
             if (l == 0) s_cnt[i] = n;
         }
@@ -255,11 +264,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p
         __syncthreads();
         for (int i = w; i < nr; i += kPagedThreads / 64) {
             if (!ended[r0 + i]) continue;
+            const int held = pages_held(r0 + i);
             long at = height + s_cnt[i];
             for (int j0 = 0; j0 < p.max_pages; j0 += 64) {
                 const int j = j0 + l;
                 const size_t cell = (size_t)(r0 + i) * p.max_pages + j;
-                const int id = j < p.max_pages ? owned_page(p.owned[cell]) : -1;
+                const int id = j < p.max_pages ? own(r0 + i, j, held) : -1;
                 const unsigned long long has = __ballot(page_ok(id, p.n_pages));
                 const long to = at + __popcll(has & ((1ull << l) - 1));
                 if (page_ok(id, p.n_pages) && to < p.n_pages) p.free_pages[to] = id;
@@ -313,10 +323,10 @@ __global__ __launch_bounds__(TH) void paged_reorder_plan_kernel(PagedDev p, cons
         const int j = len >> p.page_shift;
         if (j < old >> p.page_shift) *flags |= kShorter;
         if ((len & mask) == 0) return false;
-        const int own = owned_page(p.owned[(size_t)from * p.max_pages + j]);
+        const int own = owned_page(p.owned[(size_t)from * p.max_pages + j], true);
         if (!page_ok(own, p.n_pages) || own != p.table[(size_t)from * p.max_pages + j]) *flags |= kNotOwned;
         x->mine = p.owned[(size_t)row * p.max_pages + j];
-        return !page_ok(owned_page(x->mine), p.n_pages);
+        return !page_ok(owned_page(x->mine, j < pages_of(old, p.page_shift)), p.n_pages);
     };
     const bool one = p.n_requests <= per;  // (one pass: what it finds is kept)
     Row x{};
@@ -381,9 +391,13 @@ __global__ __launch_bounds__(TH) void paged_reorder_plan_kernel(PagedDev p, cons
                 const int id = p.free_pages[n_free - 1 - at];
                 cells[held - 1] = page_ok(id, p.n_pages) ? id : -1;
             } else if (x.mine <= -2) {  // come back to the page that it went back from
-                cells[held - 1] = owned_page(x.mine);
+                cells[held - 1] = owned_page(x.mine, true);
             }
-            if (held < pages_of(x.old, p.page_shift) && cells[held] >= 0) cells[held] = -2 - cells[held];  // goes back from it
+            const int had = pages_of(x.old, p.page_shift);
+            if (held < had && cells[held] >= 0) cells[held] = -2 - cells[held];  // goes back from it
+            // (what a dropped step left in the places that the row now reaches; steps leave it without a gap)
+            for (int j = had; j < x.len >> p.page_shift && cells[j] != -1; ++j)
+                if (cells[j] >= 0) cells[j] = -1;
             lens_out[row] = x.len;
         }
         taken += sum;
@@ -453,7 +467,7 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(PagedDev p, jk_kv_q8 c,
         const int row = row0 + b, from = parent_row(parent, row, width), len = p.lens[row];
         if (from == row || len <= 0 || len > cap || (len & mask) == 0) continue;
         const int j = len >> p.page_shift;
-        const int src = owned_page(p.owned[(size_t)from * p.max_pages + j]);
+        const int src = owned_page(p.owned[(size_t)from * p.max_pages + j], true);
         const int dst = p.owned[(size_t)row * p.max_pages + j];
         if (!page_ok(src, p.n_pages) || !page_ok(dst, p.n_pages) || i * 16 >= (len & mask) * hd) continue;
         moves[b] = true;

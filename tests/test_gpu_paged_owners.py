@@ -90,7 +90,7 @@ def both(d, p, h, width, calls, check=True):
             O.check(p, h, width)
 
 
-@pytest.mark.parametrize("unequal,drafts", [(False, False), (True, False)])
+@pytest.mark.parametrize("unequal,drafts", [(False, False), (True, False), (False, True), (True, True)])
 @pytest.mark.parametrize("groups,width,max_pages,n_steps", [(1, 1, 8, 30), (1, 4, 8, 40), (3, 8, 12, 30), (2, 13, 8, 20),
                                                             (90, 4, 12, 8), (1, 32, 1030, 8)])
 def test_random_sequences(gpu, groups, width, max_pages, n_steps, unequal, drafts):
@@ -102,7 +102,7 @@ def test_random_sequences(gpu, groups, width, max_pages, n_steps, unequal, draft
         both(d, p, h, width, O.steps(rng, groups, width, 16, max_pages, n_steps, unequal, drafts), check=b <= 32)
 
 
-@pytest.mark.parametrize("drafts", [False])
+@pytest.mark.parametrize("drafts", [False, True])
 @pytest.mark.parametrize("groups,width", [(300, 4), (206, 5), (75, 16)])
 def test_batches_of_several_passes(gpu, groups, width, drafts):
     """More requests than the planning workgroup takes at once."""
@@ -111,6 +111,39 @@ def test_batches_of_several_passes(gpu, groups, width, drafts):
     d = Dev(gpu, b, 9, n_pages, 16, b * 40)
     p, h = O.Owners(b, 9, n_pages, 16), O.Held(b, n_pages, 16)
     both(d, p, h, width, O.steps(rng, groups, width, 16, 9, 4, True, drafts), check=False)
+
+
+def test_dropped_step_then_release(gpu):
+    """The pages of a dropped step are free again, whoever gets them next: no page has two owners or is free twice."""
+    d, p, h = Dev(gpu, 3, 8, 12, 16, 64), O.Owners(3, 8, 12, 16), O.Held(3, 12, 16)
+    both(d, p, h, 1, [("extend", [16, 16, 0]), ("draft", [5, 0, 0]), ("extend", [0, 1, 0]), ("release", [1, 0, 0]),
+                      ("extend", [0, 0, 40]), ("release", [0, 1, 1])])
+    assert sorted(d.free.tolist()) == list(range(12)) and int(d.n_free) == 12
+
+
+def test_dropped_step_then_release_of_one_table(gpu):
+    """The same where table and owned are one array."""
+    torch = gpu
+    d = Dev(torch, 2, 4, 6, 16, 64)
+    d.p = jk.paged(d.lens, d.table, d.table, d.free, d.n_free, 16)
+    jk.dev_paged_reset(d.p)
+    d.extend([16, 16])
+    d.extend([20, 0], drop=True)
+    d.extend([0, 1])
+    assert int(d.n_free) == 3
+    jk.dev_paged_release(d.p, d.dev([1, 0]))
+    assert int(d.n_free) == 4
+    in_use = set(d.table[1, :2].tolist())
+    assert len(in_use) == 2 and sorted(d.free.tolist()[:4] + list(in_use)) == list(range(6))
+
+
+def test_dropped_step_then_reordering(gpu):
+    """A page that a dropped step left in a row's place is not the row's to fill: another request may have it."""
+    d, p, h = Dev(gpu, 4, 4, 16, 16, 64), O.Owners(4, 4, 16, 16), O.Held(4, 16, 16)
+    both(d, p, h, 2, [("extend", [16, 0, 20, 0]), ("reorder", [0, 0, 0, 0]), ("draft", [4, 4, 0, 0]),
+                      ("extend", [0, 0, 16, 16]), ("draft", [0, 30, 0, 0]), ("extend", [3, 0, 0, 0]), ("reorder", [0, 0, 1, 0]),
+                      ("release", [1, 1, 0, 0]), ("extend", [0, 0, 5, 5]), ("release", [0, 0, 1, 1])])
+    assert int(d.n_free) == 16
 
 
 @pytest.mark.parametrize("lens,parents", [([17, 15], [1, 0]), ([16, 15], [1, 0]), ([33, 20, 20], [1, 0, 2])])
