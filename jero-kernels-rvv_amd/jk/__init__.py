@@ -828,17 +828,20 @@ _dtype_codes = {}  # the same by dtype object, filled as they are met (a name co
 
 
 class PagedC(C.Structure):
+    on_host = False  # whether one of its tensors lies in host memory (_held)
     _fields_ = [("n_requests", _sz), ("max_pages", _sz), ("n_pages", _sz), ("page", _sz), ("lens", _vp),
                 ("table", _vp), ("owned", _vp), ("free_pages", _vp), ("n_free", _vp)]
 
 
 class PagedStepC(C.Structure):
+    on_host = False
     requests_held = None  # that q_start has room for, where that is known
     _fields_ = [("max_tokens", _sz), ("q_start", _vp), ("slots", _vp), ("positions", _vp), ("requests", _vp),
                 ("status", _vp)]
 
 
 class KvQ8C(C.Structure):
+    on_host = False
     _fields_ = [("n_pages", _sz), ("page", _sz), ("n_kv", _sz), ("head_dim", _sz), ("k", _vp), ("v", _vp),
                 ("k_scale", _vp), ("v_scale", _vp)]
 
@@ -848,10 +851,12 @@ class AttnQ8ArgsC(C.Structure):
                 ("q_stride_token", _sz), ("q_stride_head", _sz), ("out_stride_token", _sz), ("out_stride_head", _sz),
                 ("n_requests", _sz), ("max_pages", _sz), ("q_start", _vp), ("lens", _vp), ("table", _vp),
                 ("max_new", _sz), ("max_len", _sz), ("scale", C.c_float), ("window", _sz)]
+    on_host = False
     head_dim = None  # of the queries, where they are known (the C struct has the cache's)
 
 
 class BeamArgsC(C.Structure):
+    on_host = False
     _fields_ = [("logits", _vp), ("dtype", C.c_int32), ("groups", _sz), ("width", _sz), ("vocab", _sz),
                 ("stride", _sz), ("scores", _vp), ("done", _vp), ("eos", C.c_int32), ("scores_out", _vp),
                 ("parents", _vp), ("tokens", _vp), ("done_out", _vp)]
@@ -888,7 +893,19 @@ def _strides_of(shape, stride) -> tuple[int, int]:
 def _held(struct, *tensors):
     """The struct, which keeps the tensors whose addresses it holds."""
     struct.tensors = tensors
+    struct.on_host = any(x is not None and not x.is_cuda for x in tensors)
     return struct
+
+
+def _refuse_host():
+    raise TensorBoundsError("a tensor in host memory: the serving calls take device tensors")
+
+
+def _workspace(ws) -> int:
+    """Address of a device workspace (or None; an address is taken as it is)."""
+    if ws is not None and type(ws) is not int and not getattr(ws, "is_cuda", False):
+        _refuse_host()
+    return _ptr(ws)
 
 
 def _i32(*tensors):
@@ -904,6 +921,8 @@ def _ints(x, n: int) -> int:
     # (these run in every step: the table first, its filling only for a type not met yet)
     if (_dtype_codes.get(x.dtype) != _I32 and _code_of(x) != _I32) or x.numel() != n or not x.is_contiguous():
         raise TensorBoundsError(f"a packed int32 tensor of {n} elements is needed")
+    if not x.is_cuda:
+        _refuse_host()
     return x.data_ptr()
 
 
@@ -913,7 +932,8 @@ def paged(lens, table, owned, free_pages, n_free, page: int) -> PagedC:
     _i32(lens, table, owned, free_pages, n_free)
     if table.shape != owned.shape or table.dim() != 2 or table.shape[0] != lens.numel():
         raise TensorBoundsError("table and owned need one row a request and the same columns")
-    _ints(n_free, 1)
+    if n_free.numel() != 1:
+        raise TensorBoundsError("the stack's height needs a tensor of one element")
     return _held(PagedC(lens.numel(), table.shape[1], free_pages.numel(), page, _ptr(lens), _ptr(table), _ptr(owned),
                         _ptr(free_pages), _ptr(n_free)), lens, table, owned, free_pages, n_free)
 
@@ -923,7 +943,8 @@ def paged_step(q_start, slots, positions, requests, status) -> PagedStepC:
     _i32(q_start, slots, positions, requests, status)
     if not slots.numel() == positions.numel() == requests.numel():
         raise TensorBoundsError("slots, positions and requests need the same length")
-    _ints(status, 1)
+    if status.numel() != 1:
+        raise TensorBoundsError("the status needs a tensor of one element")
     step = _held(PagedStepC(slots.numel(), _ptr(q_start), _ptr(slots), _ptr(positions), _ptr(requests), _ptr(status)),
                  q_start, slots, positions, requests, status)
     step.requests_held = q_start.numel() - 1
@@ -932,6 +953,8 @@ def paged_step(q_start, slots, positions, requests, status) -> PagedStepC:
 
 def dev_paged_reset(p: PagedC, stream=None):
     """jk_paged_reset: empty requests, all pages free."""
+    if p.on_host:
+        _refuse_host()
     _check(lib().jk_paged_reset(stream, C.addressof(p)))
 
 
@@ -940,6 +963,8 @@ def dev_paged_extend(p: PagedC, n_new, step: PagedStepC, lens_out=None, n_free_o
     n = p.n_requests
     if step.requests_held not in (None, n):
         raise TensorBoundsError("the step's q_start needs one element more than there are requests")
+    if p.on_host or step.on_host:
+        _refuse_host()
     status = (_lib_handle or lib()).jk_paged_extend(stream, C.addressof(p), _ints(n_new, n), C.addressof(step),
                                                     _ints(lens_out, n), _ints(n_free_out, 1))
     if status:
@@ -948,11 +973,15 @@ def dev_paged_extend(p: PagedC, n_new, step: PagedStepC, lens_out=None, n_free_o
 
 def dev_paged_release(p: PagedC, ended, stream=None):
     """jk_paged_release: the pages of the requests with ended[r] != 0 back on the stack."""
+    if p.on_host:
+        _refuse_host()
     _check(lib().jk_paged_release(stream, C.addressof(p), _ints(ended, p.n_requests)))
 
 
 def dev_paged_reorder(p: PagedC, parent, width: int, status, lens_out=None, table_out=None, stream=None):
     """jk_paged_reorder: row r of each group of `width` goes on from row parent[r]."""
+    if p.on_host:
+        _refuse_host()
     n = p.n_requests
     failed = (_lib_handle or lib()).jk_paged_reorder(stream, C.addressof(p), _ints(parent, n), width, _ints(status, 1),
                                                      _ints(lens_out, n), _ints(table_out, n * p.max_pages))
@@ -980,8 +1009,11 @@ def dev_kv_append_q8(c: KvQ8C, k, v, slots, stream=None):
     n, kv, hd = shape
     if kv != c.n_kv or hd != c.head_dim:
         raise TensorBoundsError("keys of the cache's heads are needed")
-    status = (_lib_handle or lib()).jk_kv_append_q8(stream, C.addressof(c), k.data_ptr(), v.data_ptr(), _dtype_of(k), n, st,
-                                                    sh, _ints(slots, n))
+    dtype = _dtype_of(k)
+    if c.on_host or not (k.is_cuda and v.is_cuda):
+        _refuse_host()
+    status = (_lib_handle or lib()).jk_kv_append_q8(stream, C.addressof(c), k.data_ptr(), v.data_ptr(), dtype, n, st, sh,
+                                                    _ints(slots, n))
     if status:
         _check(status)
 
@@ -994,7 +1026,11 @@ def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
         if x is not None:
             if x.numel() != elements or not x.is_contiguous() or (dtype is not None and x.dtype != dtype):
                 raise TensorBoundsError("outputs need packed tensors [slots][kv heads][head_dim] of one type")
+            if not x.is_cuda:
+                _refuse_host()
             dtype, first = x.dtype, x
+    if c.on_host:
+        _refuse_host()
     status = (_lib_handle or lib()).jk_kv_read_q8(stream, C.addressof(c), _ints(slots, n), n,
                                                   F32 if dtype is None else _dtype_of(first),
                                                   0 if k_out is None else k_out.data_ptr(),
@@ -1005,6 +1041,8 @@ def dev_kv_read_q8(c: KvQ8C, slots, k_out, v_out, stream=None):
 
 def dev_kv_reorder_q8(c: KvQ8C, p: PagedC, parent, width: int, status, stream=None):
     """jk_kv_reorder_q8: the cache's part of dev_paged_reorder, after it, for each layer."""
+    if c.on_host or p.on_host:
+        _refuse_host()
     _check(lib().jk_kv_reorder_q8(stream, C.addressof(c), C.addressof(p), _ints(parent, p.n_requests), width,
                                   _ints(status, 1)))
 
@@ -1034,7 +1072,10 @@ def dev_attn_q8(c: KvQ8C, a: AttnQ8ArgsC, ws=None, stream=None, ws_bytes=None):
     """jk_attn_q8: causal attention of the step's queries over the paged 8-bit cache."""
     if a.head_dim is not None and a.head_dim != c.head_dim:
         raise TensorBoundsError(f"queries of {a.head_dim} channels for a cache of {c.head_dim}")
-    status = (_lib_handle or lib()).jk_attn_q8(stream, C.addressof(c), C.addressof(a), _ptr(ws), _ws_bytes(ws, ws_bytes))
+    if c.on_host or a.on_host:
+        _refuse_host()
+    status = (_lib_handle or lib()).jk_attn_q8(stream, C.addressof(c), C.addressof(a), _workspace(ws),
+                                               _ws_bytes(ws, ws_bytes))
     if status:
         _check(status)
 
@@ -1066,7 +1107,9 @@ def beam_workspace_bytes(a: BeamArgsC) -> int:
 
 def dev_beam_select(a: BeamArgsC, ws, stream=None, ws_bytes=None):
     """jk_beam_select: the width best continuations of each group's hypotheses."""
-    _check(lib().jk_beam_select(stream, C.addressof(a), _ptr(ws), _ws_bytes(ws, ws_bytes)))
+    if a.on_host:
+        _refuse_host()
+    _check(lib().jk_beam_select(stream, C.addressof(a), _workspace(ws), _ws_bytes(ws, ws_bytes)))
 
 
 def dev_measure_stream_read(buf, nbytes, sink, stream=None):
