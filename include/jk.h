@@ -664,7 +664,7 @@ typedef struct jk_attn_q8_args {
     size_t n_tokens; /* rows of q and out; those that q_start gives to no request are left as they are */
     size_t n_heads;  /* a multiple of n_kv */
     size_t q_stride_token, q_stride_head, out_stride_token, out_stride_head;
-    size_t n_requests, max_pages;
+    size_t n_requests, max_pages; /* max_pages * page at most 2^31 - 4096 */
     const int32_t *q_start; /* [n_requests + 1] */
     const int32_t *lens;    /* [n_requests], the step's tokens included; not past max_pages * page */
     const int32_t *table;   /* [n_requests][max_pages] */

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
     if (c0 >= cols || cols > a.few_cols) return;
     const Span sp = span_of(a, rq, c0, min(c0 + 16, cols));
     if (split >= sp.active) return;
-    const int begin = sp.lo + split * sp.chunk, end = min(sp.hi, begin + sp.chunk);
+    const int begin = sp.lo + split * sp.chunk, end = piece_end(sp, begin);
 
     f32x4 o[NT];
 #pragma unroll
@@ -377,7 +377,7 @@ static jk_status attn_check(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
     if (a->n_heads == 0 || a->n_heads % c->n_kv || a->n_heads > 65536)
         return fail(JK_TENSOR_BOUNDS, "attn_q8: %zu query heads for %zu kv heads", a->n_heads, c->n_kv);
     if (a->n_requests == 0 || a->max_pages == 0 || a->n_requests > (size_t)INT32_MAX / 64 ||
-        a->max_pages > (size_t)INT32_MAX / c->page)
+        a->max_pages > kMaxTokens / c->page)
         return fail(JK_TENSOR_BOUNDS, "attn_q8: %zu requests of %zu pages", a->n_requests, a->max_pages);
     if (a->n_tokens > (size_t)INT32_MAX / a->n_heads)
         return fail(JK_TENSOR_BOUNDS, "attn_q8: %zu tokens of %zu heads exceed the int32 range", a->n_tokens, a->n_heads);
@@ -412,7 +412,7 @@ static AttnPlan attn_plan(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
     if (a->window) len = std::min(len, a->window + new_tokens);
     auto cut = [&](size_t share, size_t least, size_t *splits, size_t *chunk) {
         *chunk = std::max({share, len <= kWholeLen ? kWholeLen : least, (len + kMaxSplits - 1) / kMaxSplits});
-        *chunk = (*chunk + 127) / 128 * 128;
+        *chunk = (std::min(*chunk, std::max<size_t>(len, 1)) + 127) / 128 * 128;
         *splits = std::max<size_t>(1, (len + *chunk - 1) / *chunk);
     };
     const size_t few = a->dtype == JK_F32 ? kFewColsF32 : kFewCols;

@@ -73,6 +73,8 @@ __device__ __forceinline__ Req request_of(const AttnDev &a, int r) {
 // The keys that columns [c0, c1) of a request can see, [lo, hi) with lo a multiple of 64, cut into pieces of
 // `chunk` (a multiple of 128): the plan's, or longer ones where more than `splits` pieces would be needed.
 constexpr int kMaxSplits = 256;
+// Tokens of a request end so far below 2^31 that what is added to their numbers (tiles ahead, roundings) stays an int.
+constexpr size_t kMaxTokens = ((size_t)1 << 31) - 4096;
 struct Span {
     int lo, hi, chunk, active;
 };
@@ -83,9 +85,11 @@ __device__ __forceinline__ Span span_of(const AttnDev &a, const Req &q, int c0, 
     s.hi = max(min(q.len, p1 + 1), s.lo);
     const int n = s.hi - s.lo;
     s.chunk = max(a.chunk, ((n + a.splits - 1) / a.splits + 127) & ~127);
-    s.active = max(1, (n + s.chunk - 1) / s.chunk);
+    s.active = max(1, (int)(((unsigned)n + s.chunk - 1) / s.chunk));
     return s;
 }
+// The end of the piece that begins at `begin`.
+__device__ __forceinline__ int piece_end(const Span &s, int begin) { return s.hi - begin > s.chunk ? begin + s.chunk : s.hi; }
 
 // Two biased codes (code + 128 in the low byte of each half) as f16 pair code / 512: a half 0x00bb is the
 // subnormal bb * 2^-24, and bb * 2^-24 * 2^15 - 128 / 512 = code / 512 exactly.

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     if (cols <= a.few_cols || c0 >= cols) return;
     const Span sp = span_of(a, rq, c0, min(c0 + a.tile_cols, cols));
     if (split >= sp.active) return;
-    const int begin = sp.lo + split * sp.chunk, end = min(sp.hi, begin + sp.chunk);
+    const int begin = sp.lo + split * sp.chunk, end = piece_end(sp, begin);
 
     // this lane's columns
     const int w0 = c0 + w * (32 * NC);  // the wave's first
