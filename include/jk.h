@@ -684,7 +684,7 @@ jk_status jk_attn_q8(jk_stream s, const jk_kv_q8 *c, const jk_attn_q8_args *a, v
 
 /* One step of beam search over `groups` groups of `width` hypotheses. The total of token t after hypothesis b is
  * score_b + (x_bt - m_b - log(sum_u exp(x_bu - m_b))), m_b the row's largest logit; NaN logits count as -inf and a
- * total that is NaN as -inf. A finished hypothesis (done != 0) goes on only as itself: token eos, its score as it is. The
+ * total that is NaN as -inf. A finished hypothesis (done != 0) goes on only as itself: token eos, its score as its total. The
  * width best come out in order: larger total first, at equal totals the lower hypothesis, within one the larger
  * logit, at equal logits the lower token. */
 typedef struct jk_beam_args {

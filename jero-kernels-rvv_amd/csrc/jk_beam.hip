@@ -167,7 +167,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamDev a) {
         if (l < a.width) s_total[b][l] = -__builtin_inff(), s_tok[b][l] = -1;
         wave_lds_sync();
         if (a.done && a.done[row]) {
-            if (l == 0) s_total[b][0] = a.scores[row], s_tok[b][0] = a.eos;
+            const float t = a.scores[row];
+            if (l == 0) s_total[b][0] = __builtin_isnan(t) ? -__builtin_inff() : t, s_tok[b][0] = a.eos;
             continue;
         }
         const float score = a.scores[row];
