@@ -235,7 +235,7 @@ __global__ __launch_bounds__(256) void paged_reset_kernel(PagedDev p) {
 // requests with 128 columns 16 us. Requests end rarely; a launch over many CUs would need a second one for the places.
 __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p, const int32_t *__restrict__ ended) {
     __shared__ unsigned long long s_scan[17];
-    __shared__ int s_cnt[kPagedThreads];
+    __shared__ int s_cnt[kPagedThreads], s_held[kPagedThreads];  // pages that an ended request owns; that it uses (-1: goes on)
     const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
     long height = min(max(*p.n_free, 0), p.n_pages);
     auto pages_held = [&](int r) { return min(pages_of(max(p.lens[r], 0), p.page_shift), p.max_pages); };
@@ -248,12 +248,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p
         const int nr = min(kPagedThreads, p.n_requests - r0);
         for (int i = w; i < nr; i += kPagedThreads / 64) {
             int n = 0;
-            if (ended[r0 + i]) {
-                const int held = pages_held(r0 + i);
+            const int held = pages_held(r0 + i);  // (its load goes out beside that of the flag)
+            const bool ends = ended[r0 + i] != 0;
+            if (ends)
                 for (int j = l; j < p.max_pages; j += 64) n += page_ok(own(r0 + i, j, held), p.n_pages);
-            }
             n = wave_sum64_dpp(n);
-            if (l == 0) s_cnt[i] = n;
+            if (l == 0) s_cnt[i] = n, s_held[i] = ends ? held : -1;
         }
         __syncthreads();
         const int mine = tid < nr ? s_cnt[tid] : 0;
@@ -263,8 +263,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p
         if (tid < nr) s_cnt[tid] = before;
         __syncthreads();
         for (int i = w; i < nr; i += kPagedThreads / 64) {
-            if (!ended[r0 + i]) continue;
-            const int held = pages_held(r0 + i);
+            const int held = s_held[i];
+            if (held < 0) continue;
             long at = height + s_cnt[i];
             for (int j0 = 0; j0 < p.max_pages; j0 += 64) {
                 const int j = j0 + l;
