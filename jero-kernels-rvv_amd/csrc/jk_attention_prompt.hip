@@ -11,10 +11,10 @@ namespace jk {
 //      8 channels of token lane % 32.
 //   V: [channel][64 tokens], the tokens of each 16 ordered 0-3, 8-11, 4-7, 12-15: a lane of the second product (rows =
 //      channels) reads the 8 tokens whose scores the first one left in that half of the wave.
-// A prompt of 4096 tokens, 32 query and 8 kv heads of 128, bf16: 156 us, 880 TFLOP/s of the products under the diagonal, where a
+// A prompt of 4096 tokens, 32 query and 8 kv heads of 128, bf16: 152 us, 900 TFLOP/s of the products under the diagonal, where a
 // large matrix product reaches 1185. What bounds it: each 32 x 32 x 16 instruction needs 1 KB from LDS, which gives 64 to 67
-// bytes a cycle to a CU however it is read; that is 4096 of the about 5000 cycles of a tile, and beside it run the matrix units
-// (2048) and the exponentials, sums and conversions (about 3200 on each SIMD). 64 columns a wave would halve the reads, but need all
+// bytes a cycle to a CU however it is read; that is 4096 of the about 4600 cycles of a tile, and beside it run the matrix units
+// (2048) and the exponentials, sums and conversions (about 2800 on each SIMD). 64 columns a wave would halve the reads, but need all
 // registers of a SIMD for one wave, whose latencies then stand open (230 us). Keys kept as bytes in LDS save a quarter of the
 // reads and cost as much in unpacking (164 us).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -210,12 +210,14 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
     auto use = [&](int t0, int buf, const Pages &pages) __attribute__((always_inline)) {
         Scores s[2][NC];
         scores(buf, s);
-        float vs[NC][PG], f[NC][PG];
+        float vtop[NC];  // the largest value scale of the pages that the column sees
         bool whole = t0 + 63 <= pos_lo && pos_hi - t0 < a.window;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) vtop[c] = 0.0f;
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) vs[c][i] = pages.vs[i], f[c][i] = pages.ks[i] * to_score[c];
+            for (int c = 0; c < NC; ++c) vtop[c] = fmaxf(vtop[c], pages.vs[i]);
             whole = whole && pages.head[i] >= 0;
         }
         if (!whole) {
@@ -235,37 +237,38 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             // (a page that a column sees nothing of has no say in its references: its scales, or those of what stands in for a
             // missing page, may be of any size, or no numbers)
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c) {
+                vtop[c] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < PG; ++i) {
                     const int behind = pos[c] - (t0 + kSpan * i);
                     const bool seen = pages.head[i] >= 0 && behind >= 0 && behind - (kSpan - 1) < a.window;
-                    vs[c][i] = seen ? vs[c][i] : 0.0f;
-                    f[c][i] = seen ? f[c][i] : 0.0f;
+                    vtop[c] = fmaxf(vtop[c], seen ? pages.vs[i] : 0.0f);
                 }
+            }
         }
-        // scores are s * f, f one number a group and positive (0 becomes next to nothing: an unseen -inf stays one)
+        // scores are s * f, f one number a group and positive (0 and no numbers become next to nothing: an unseen -inf stays one)
+        float f[NC][PG];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float top = kNegInf, vtop = 0.0f;
+            float top = kNegInf;
 #pragma unroll
             for (int i = 0; i < PG; ++i) {
-                vtop = fmaxf(vtop, vs[c][i]);
-                f[c][i] = f[c][i] < 1e-37f ? 1e-37f : f[c][i];
+                f[c][i] = fmaxf(pages.ks[i] * to_score[c], 1e-37f);
                 float big = kNegInf;
 #pragma unroll
                 for (int e = 0; e < 32 / PG; ++e) big = fmaxf(big, s[(32 / PG * i + e) / 16][c].v[(32 / PG * i + e) % 16]);
                 top = fmaxf(top, big * f[c][i]);
             }
-            const bool vmove = vtop > vref[c] * kSlackV;
+            const bool vmove = vtop[c] > vref[c] * kSlackV;
             if (__any(vmove || top > m[c] + kSlack)) {
                 top = max_halves(top);
                 const float m_new = top > m[c] + kSlack ? top : m[c];
                 // (the first reference of a column comes from nothing: nothing is kept)
                 const float fade = m_new == m[c] ? 1.0f : exp2_fast(m[c] - m_new);
-                const float fade_o = vmove ? fade * (vref[c] / vtop) : fade;
+                const float fade_o = vmove ? fade * (vref[c] / vtop[c]) : fade;
                 m[c] = m_new;
-                vref[c] = vmove ? vtop : vref[c];
+                vref[c] = vmove ? vtop[c] : vref[c];
                 per[c] = kWeight / vref[c];
                 lsum[c] *= fade;
 #pragma unroll
@@ -284,7 +287,9 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             constexpr bool kInExponent = PARTS == 1;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const float vs_per = vs[c][i * PG / 4] * per[c], vw = kInExponent ? fmaxf(vs_per, kWeight * 0x1p-60f) : vs_per;
+                // (at most that, where any of it is seen)
+                const float vs_per = fminf(pages.vs[i * PG / 4] * per[c], kWeight * kSlackV);
+                const float vw = kInExponent ? fmaxf(vs_per, kWeight * 0x1p-60f) : vs_per;
                 const float shift = kInExponent ? __builtin_amdgcn_logf(vw) : 0.0f;
                 const float back = kInExponent ? __builtin_amdgcn_rcpf(vw) : 1.0f;
                 const float off = shift - (m[c] == kNegInf ? 0.0f : m[c]);
