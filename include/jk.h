@@ -639,7 +639,8 @@ typedef struct jk_kv_q8 {
  * (elements; strides of 0: packed). A page's scale d is (largest finite |x| of its tokens) / 127, and its
  * codes are round(x / d) with x * (1 / d) in f32, ties to even. A page that was begun earlier keeps its scale while it
  * suffices; when a larger value comes, its older codes become round(code * (d_old / d)). Its row 0
- * begins a page anew. Non-finite values are stored as 0, and so is a page whose largest value is below 2^-119.
+ * begins a page anew. Tokens of a step that is dropped leave the page's scale as large as they needed it, and its older codes
+ * rounded to that scale. Non-finite values are stored as 0, and so is a page whose largest value is below 2^-119.
  * The tokens of one page have to be neighbours in the step, in the order of their rows (as jk_paged_extend
  * numbers them); slots out of range, -1 among them, are skipped. */
 jk_status jk_kv_append_q8(jk_stream s, const jk_kv_q8 *c, const void *k, const void *v, int dtype, size_t n_tokens,
@@ -669,13 +670,14 @@ typedef struct jk_attn_q8_args {
     const int32_t *lens;    /* [n_requests], the step's tokens included; not past max_pages * page */
     const int32_t *table;   /* [n_requests][max_pages] */
     size_t max_new; /* bound of the new tokens of one request: later ones are left as they are */
-    size_t max_len; /* expected bound of lens: work is split by it, results do not depend on it */
+    size_t max_len; /* expected bound of lens: work is split by it, results depend on it by the order of their sums alone */
     float scale;
     size_t window; /* 0: none */
 } jk_attn_q8_args;
 /* Queries of f32 are multiplied as two f16 parts (22 bits of each row's largest value) and so are the
  * probabilities; f16 and bf16 queries are exact (to 2^-24 of their row's largest value), with
- * probabilities in f16. Scores, maxima, sums and outputs are f32 until the one rounding to dtype. The workspace holds
+ * probabilities in one f16 (2^-11 of each; who needs more calls with f32). Scores, maxima, sums and outputs are
+ * f32 until the one rounding to dtype. The workspace holds
  * the parts of rows whose keys are split over workgroups: jk_attn_q8_workspace_bytes(c, a) bytes (possibly
  * 0, then it may be NULL), 16-byte aligned, of any content; calls that share one must not overlap. */
 size_t jk_attn_q8_workspace_bytes(const jk_kv_q8 *c, const jk_attn_q8_args *a);

@@ -14,8 +14,8 @@ namespace jk {
 // channels (HDP / 16) n + t of the eight tokens whose scores it holds, so that the loads of a wave cover whole rows
 // and nothing goes through LDS.
 // What bounds it: the cache's bytes, 2 a channel and token for all columns of the group, where requests are many (64 requests,
-// 290 thousand tokens, 8 kv heads of 128, bf16: 117 us, 5.2 TB/s, as fast as a copy); where one long request is cut
-// over the CUs, a tile's chain of loads, products and exponentials (32 thousand tokens 21 us, 3.2 TB/s, and 4 for the joining); and
+// 290 thousand tokens, 8 kv heads of 128, bf16: 117-119 us, 5.1 TB/s, as fast as a copy); where one long request is cut
+// over the CUs, a tile's chain of loads, products and exponentials (32 thousand tokens 20-21 us, 3.3 TB/s, and 4 for the joining); and
 // with hundreds of columns the matrix units, of which a tile of 16 columns uses a quarter of what the prompt kernel's does. Waves
 // take tokens in turn and not columns because the few columns of a step are one tile, and its keys' loads need many
 // waves in flight: three a SIMD.
@@ -136,7 +136,6 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 3 : 1) void attn_q8_rows_kernel(A
             for (int p = 0; p < PARTS; ++p) qf[p][j] = part[p];
         }
     }
-
 
     const int pos_lo = rq.len - rq.count + c0 / a.grp, pos_hi = rq.len - rq.count + (min(c0 + 16, cols) - 1) / a.grp;
     auto use = [&](int t0, Tile &x) {
@@ -386,7 +385,9 @@ static jk_status attn_check(const jk_kv_q8 *c, const jk_attn_q8_args *a) {
 
 // How a call is cut up. Requests of up to kFewCols columns go to the rows kernel, sixteen columns a workgroup; longer ones to
 // the prompt kernel. (One request, 32 query and 8 kv heads of 128, bf16, rows against prompt kernel: 128 new tokens after 2000 20 and
-// 30 us; 512 after none 19 and 20 us, after 4000 105 and 70 us; 2048 after none 115 and 64 us.) A call that can hold both
+// 30 us; 512 after none 19 and 20 us, after 4000 105 and 70 us; 2048 after none 115 and 64 us. In f32, whose parts cost the prompt
+// kernel's products twice as much: 256 new tokens after none 10.5 and 18 us, after 2000 34 and 50, after 8000 103 and 113; 512 after
+// none 20 and 27, after 2000 64 and 64, after 8000 200 and 153; 1024 after none 45 and 46, after 2000 131 and 150.) A call that can hold both
 // launches both (the counts are known on the device only), except that the prompt kernel takes a lone request
 // whatever its length turns out to be.
 // The prompt kernel takes 256 columns a workgroup (one a CU, 159 us for the 4096-token prompt, 175 with 128) where

@@ -131,7 +131,9 @@ __device__ __forceinline__ float max_rows(float v) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Eight f32 values as f16 (PARTS 1), or as two f16 that add up to 22 bits of them. The low part is taken from the very
+// Eight f32 values as f16 (PARTS 1), or as two f16 that add up to 22 bits of them. One part for 16-bit types: a weight is then off
+// by up to 2^-11 of itself, as much as an f16 output by its own rounding (an eighth of a bf16 one's), and a second part would double the
+// matrix instructions of the second product. The low part is taken from the very
 // number that the high part became: the empty asm keeps the compiler from converting y a second time with another
 // instruction, which was seen to round some values to the other neighbour.
 template <int PARTS>

@@ -13,7 +13,7 @@ namespace jk {
 //      channels) reads the 8 tokens whose scores the first one left in that half of the wave.
 // A prompt of 4096 tokens, 32 query and 8 kv heads of 128, bf16: 152 us, 900 TFLOP/s of the products under the diagonal, where a
 // large matrix product reaches 1185. What bounds it: each 32 x 32 x 16 instruction needs 1 KB from LDS, which gives 64 to 67
-// bytes a cycle to a CU however it is read; that is 4096 of the about 4600 cycles of a tile, and beside it run the matrix units
+// bytes a cycle to a CU however it is read; that is 4096 of the about 4700 cycles of a tile, and beside it run the matrix units
 // (2048) and the exponentials, sums and conversions (about 2800 on each SIMD). 64 columns a wave would halve the reads, but need all
 // registers of a SIMD for one wave, whose latencies then stand open (230 us). Keys kept as bytes in LDS save a quarter of the
 // reads and cost as much in unpacking (164 us).
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * NW, HDP <= 128 ? 2 : 1) void attn_q8_prompt_ke
             for (int i = 1; i < PG; ++i) {
                 size_t other = place[i];
                 // (kept a value: a choice among an array's elements puts the array into scratch memory; 2048 tokens in pages of 16
-                // took 110 us so, and 91 now, in pages of 64 64)
+                // took 110 us so, and 83 now, in pages of 64 60)
                 asm("" : "+s"(other));
                 at = token >= kSpan * i ? other : at;
             }

@@ -94,7 +94,7 @@ __device__ __forceinline__ void write_token(const StepDev &st, int t, int slot, 
 
 // The plan of a step by TH threads. FILL: this launch also numbers the tokens (few of them: one launch for a decode step).
 // Its bytes are a few a request; what it takes is the latency of its rounds: the counts, their sums over the
-// workgroup, a page's place found by bisection, the stack. A step of 4 requests 4.3 us, 96 prompts (49 thousand tokens, 1500
+// workgroup, a page's place found by bisection, the stack. A step of 4 requests 4.4 us, 96 prompts (49 thousand tokens, 1500
 // pages) 8 us and their numbering 3.5, 128 requests of 7990 tokens (16 thousand pages, the largest share two stores a page)
 // 19 and 7.5.
 template <bool FILL, int TH>
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void paged_reset_kernel(PagedDev p) {
 
 // One workgroup. Each wave counts the owned pages of its requests, a prefix sum places them, and the wave
 // writes them in order of their places. Every cell of both tables goes through the one CU, a request a wave at a time: 128
-// requests with 128 columns 16 us. Requests end rarely; a launch over many CUs would need a second one for the places.
+// requests with 128 columns 17 us. Requests end rarely; a launch over many CUs would need a second one for the places.
 __global__ __launch_bounds__(kPagedThreads) void paged_release_kernel(PagedDev p, const int32_t *__restrict__ ended) {
     __shared__ unsigned long long s_scan[17];
     __shared__ int s_cnt[kPagedThreads], s_held[kPagedThreads];  // pages that an ended request owns; that it uses (-1: goes on)
@@ -295,7 +295,7 @@ __device__ __forceinline__ int parent_row(const int32_t *parent, int row, int wi
 // all read before one of them is written.
 // TABLE: it also writes the tables, of few cells (one launch instead of two).
 // Latency again: parents, lengths, the page's owner, the stack, the table, each a round of loads that waits for the one before.
-// Rows that take a page are counted by ballots, their sums over the waves with one barrier. One group of 4 rows 3.4 us (256
+// Rows that take a page are counted by ballots, their sums over the waves with one barrier. One group of 4 rows 3.7 us (256
 // threads; 5.9 with 1024, shuffles and a barrier a sum), 16 groups of 8 rows and 33 columns 5.8.
 template <int MW>
 __device__ __forceinline__ void reorder_column(const PagedDev &p, const int32_t *parent, int width, bool ok,
@@ -550,7 +550,7 @@ jk_status jk_paged_extend(jk_stream s, const jk_paged *p, const int32_t *n_new, 
     // One workgroup numbers up to this many tokens itself: a second launch costs more until there are some ten a thread (16
     // requests of 500 new tokens 10.8 us, 12.2 in two launches; 100 of 128 13.1 and 12.0).
     if (st->max_tokens <= 8 * kPagedThreads) {
-        if (p->n_requests <= 256 && st->max_tokens <= 512)  // (few waves to a barrier: a step of 4 tokens 4.3 us on the GPU, 6.8 with 1024 threads)
+        if (p->n_requests <= 256 && st->max_tokens <= 512)  // (few waves to a barrier: a step of 4 tokens 4.4 us on the GPU, 6.8 with 1024 threads)
             hipLaunchKernelGGL((paged_extend_kernel<true, 256>), dim3(1), dim3(256), 0, (hipStream_t)s, d, n_new, sd, lo,
                                fo);
         else
